@@ -495,6 +495,150 @@ int oxs_pack_q8_0(const void* w, uint32_t m, uint32_t k, void* w_packed, void* s
 int oxs_mmvq_q8_0(float* y, const void* w_packed, const void* x_q8_1, uint32_t m, uint32_t k, uint32_t batch,
                   void* stream);
 
+/*
+ * Token log probabilities: what a serving API returns beside a sampled token
+ * (its log probability, its rank, the likeliest alternatives), what scoring a
+ * prompt or a set of choices needs, and the entropy of each row. No
+ * counterpart in the reference, whose sampler keeps only the renormalised
+ * probabilities of the tokens that its filters leave.
+ *
+ * Row b's distribution is over the tokens i that are present: allowed by the
+ * mask (if any), with a logit that is neither NaN nor -inf. With
+ * y_i = cap * tanh(l_i / cap) for logit_softcap > 0 (else l_i) and
+ * z_i = y_i / temperatures[b] where that is above 1e-6 (else y_i: a row that
+ * oxs_decode_step takes the raw argmax of has its raw log probabilities):
+ *   logsumexp   lse = ln(sum_i e^(z_i))
+ *   logprob     z_t - lse; -inf for a token that is not present (an id >= vocab among them)
+ *   entropy     -sum_i p_i ln p_i, p_i = e^(z_i - lse), in nats
+ *   rank        1 + the number of present tokens with a larger l_i, or an equal l_i and a lower id;
+ *               0 for a token that is not present
+ *   alternatives  the first top_n present tokens in that order; an entry past the last present
+ *               token has id 0xffffffff and log probability -inf
+ * A row with no token present (status OXS_ROW_EMPTY) has lse -inf and entropy
+ * 0. A row whose largest present logit is +inf (without a softcap) has lse
+ * +inf, entropy NaN, log probability NaN for the +inf tokens and -inf for the
+ * others; ranks and alternatives are as above. -0.0 and +0.0 are equal.
+ * Penalties, biases and the sampler's filters are not applied.
+ */
+#define OXS_LOGPROBS_MAX_TOP 32u    /* alternatives per row */
+#define OXS_LOGPROBS_MAX_TOKENS 64u /* given tokens per row */
+
+typedef struct oxs_logprobs {
+  uint32_t rows;          /* rows (sequences of a decode step, or positions of prompts) */
+  uint32_t vocab;         /* V */
+  int32_t logits_dtype;   /* OXS_DTYPE_F32 or OXS_DTYPE_BF16 */
+  uint32_t tokens_per_row; /* T, 0 to OXS_LOGPROBS_MAX_TOKENS */
+  int64_t logits_ld;      /* elements between consecutive rows (>= vocab when rows > 1) */
+  const void* logits;     /* [rows][logits_ld], read only */
+  const uint32_t* tokens; /* [rows][tokens_ld] given token ids (may repeat); NULL when T is 0 */
+  int64_t tokens_ld;      /* >= T when rows > 1 */
+  const uint32_t* allowed_mask; /* optional, as oxs_batch.allowed_mask */
+  int64_t mask_ld;              /* as oxs_batch.mask_ld */
+  const float* temperatures;    /* optional [rows] */
+  float logit_softcap;          /* as oxs_batch.logit_softcap */
+  uint32_t top_n;               /* alternatives per row, 0 to OXS_LOGPROBS_MAX_TOP */
+  float* out_logprobs;      /* optional [rows][T] */
+  uint32_t* out_ranks;      /* optional [rows][T] */
+  float* out_logsumexp;     /* optional [rows] */
+  float* out_entropy;       /* optional [rows] */
+  uint32_t* out_top_ids;    /* optional [rows][top_n] */
+  float* out_top_logprobs;  /* optional [rows][top_n] */
+  int32_t* out_status;      /* optional [rows]: OXS_ROW_OK or OXS_ROW_EMPTY */
+  void* workspace;          /* device, 16-byte aligned, oxs_logprobs_workspace_bytes() or more; any content */
+  uint64_t workspace_bytes;
+} oxs_logprobs;
+
+/* Bytes of workspace that any oxs_token_logprobs call needs. Calls that may
+ * overlap (on different streams, or replays of different graphs) need a
+ * workspace each. */
+size_t oxs_logprobs_workspace_bytes(void);
+
+/*
+ * Computes every row of `lp` on `stream`, on the calling thread's current
+ * device. Asynchronous and stream ordered; allocates nothing and issues only
+ * kernels, so it can be captured in a HIP graph. The result of a row does not
+ * depend on timing, and ranks and alternatives are exact. rows == 0 does
+ * nothing. The outputs must not overlap the inputs or each other. Returns
+ * OXS_ERR_SHAPE_MISMATCH for vocab 0, OXS_ERR_LIMITS for T, top_n, vocab
+ * (2^30) or rows (2^23) above their limits, OXS_ERR_INVALID_ARGUMENT for
+ * missing or misaligned pointers (logits to their element, all others to 4
+ * bytes), leading dimensions that are too small, an unknown dtype or too
+ * little workspace, OXS_ERR_HIP if the launch fails.
+ */
+int oxs_token_logprobs(const oxs_logprobs* lp, void* stream);
+
+/*
+ * Low-rank adapters of many requests at once, beside the projection that they
+ * share (oxs_mmvq_q8_0): adapter i has A_i [rank_i][k], B_i [m][rank_i] and a
+ * scale s_i, and a row b with adapter a gets
+ *   y_b += B_a (s_a A_a x_b).
+ * No counterpart in the reference. The table holds the adapters of `dtype` in
+ * the layouts that the kernels read, in memory of the caller; its sizes are
+ * oxs_lora_table_bytes. Before its first use ranks[] must be zero (no slot
+ * loaded); nothing else need be initialised.
+ */
+#define OXS_DTYPE_F16 2 /* adapter weights only */
+#define OXS_LORA_MAX_RANK 256u
+#define OXS_LORA_NONE 0xffffffffu /* a row without an adapter */
+
+typedef struct oxs_lora_table {
+  uint32_t m;            /* outputs of the projection (tokens) */
+  uint32_t k;            /* its inputs (hidden size); any value >= 1 */
+  uint32_t max_adapters; /* slots, 1 to 65536 */
+  uint32_t max_rank;     /* largest rank of a slot, 1 to OXS_LORA_MAX_RANK */
+  int32_t dtype;         /* of the weights: OXS_DTYPE_F32, OXS_DTYPE_BF16 or OXS_DTYPE_F16 */
+  void* a;               /* device, 16-byte aligned */
+  void* b;               /* device, 16-byte aligned */
+  uint32_t* ranks;       /* device [max_adapters]; 0: no adapter in the slot */
+  float* scales;         /* device [max_adapters] */
+} oxs_lora_table;
+
+/* Bytes that table->a and table->b must hold, from the table's sizes and
+ * dtype (its pointers are not looked at). OXS_ERR_INVALID_ARGUMENT for sizes
+ * of 0 or above their limits (m and k: 2^30) or an unknown dtype. */
+int oxs_lora_table_bytes(const oxs_lora_table* table, size_t* a_bytes, size_t* b_bytes);
+
+/*
+ * Puts an adapter into a slot, in stream order (a captured oxs_lora_add sees
+ * it at its next replay): a is [rank][a_ld] and b is [m][b_ld], device, of
+ * the table's dtype, a_ld >= k and b_ld >= rank. rank 0 empties the slot (a
+ * and b may be NULL). Must not overlap an oxs_lora_add on another stream.
+ */
+int oxs_lora_load(const oxs_lora_table* table, uint32_t slot, const void* a, int64_t a_ld, const void* b,
+                  int64_t b_ld, uint32_t rank, float scale, void* stream);
+
+typedef struct oxs_lora_batch {
+  uint32_t batch;          /* rows */
+  int32_t x_dtype;         /* OXS_DTYPE_F32 or OXS_DTYPE_BF16 */
+  int32_t y_dtype;         /* OXS_DTYPE_F32 or OXS_DTYPE_BF16 */
+  const void* x;           /* [batch][x_ld] the projection's inputs, before any quantization */
+  int64_t x_ld;            /* >= k when batch > 1 */
+  void* y;                 /* [batch][y_ld] in/out: its outputs */
+  int64_t y_ld;            /* >= m when batch > 1 */
+  const uint32_t* adapters; /* [batch] slot of each row, OXS_LORA_NONE for none */
+  void* workspace;         /* device, 16-byte aligned; any content */
+  uint64_t workspace_bytes; /* >= oxs_lora_workspace_bytes(table, batch) */
+} oxs_lora_batch;
+
+/* Workspace of an oxs_lora_add over `batch` rows (0 for invalid sizes). Calls
+ * that may overlap need a workspace each. */
+size_t oxs_lora_workspace_bytes(const oxs_lora_table* table, uint32_t batch);
+
+/*
+ * y_b += B_a (s_a A_a x_b) for every row b with a loaded adapter a =
+ * adapters[b]; a row whose slot is empty or >= max_adapters is neither read
+ * nor written. Products are exact and sums are in 32 bits; the result is
+ * added to y in 32 bits and rounded to y_dtype once. Rows may have any
+ * adapters in any order; rows of one adapter that stand together share reads.
+ * An infinity or NaN in one adapter's weights or one row's x reaches no row
+ * but those of that adapter and that row. Asynchronous and stream ordered on
+ * the current device; allocates nothing and issues only kernels. Returns
+ * OXS_ERR_INVALID_ARGUMENT for missing or misaligned pointers, too small
+ * leading dimensions or workspace or unknown dtypes, OXS_ERR_LIMITS for
+ * batch above 65536 or batch * m above 2^31, OXS_ERR_HIP if a launch fails.
+ */
+int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* batch, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -1,6 +1,6 @@
 """Python view of the MI355X batched token sampler (liboxide_sampler.so).
 
-Four layers, all thin over the C ABI in include/oxide_sampler.h:
+Layers, all thin over the C ABI in include/oxide_sampler.h:
 
 - `BatchSampler`: the batched device call, `oxs_sample_batch`, on torch
   tensors that already live on the GPU (the decode-loop form).
@@ -12,6 +12,10 @@ Four layers, all thin over the C ABI in include/oxide_sampler.h:
 - `DecodeLoop`: the scheduler's decode stage
   (crates/oxide-engine/src/continuous_batching.rs:940-1040) with every
   sequence's sampler state on the device, one `oxs_decode_step` per step.
+- `LmHeadQ8_0` and `quantize_q8_1`: the LM head in front of the sampler, with
+  `LoraAdapters` (`oxs_lora_add`) beside it for requests with adapters.
+- `TokenLogprobs`: log probabilities, ranks, entropy and alternatives of the
+  same logits (`oxs_token_logprobs`).
 
 There is no CPU path: without the built library every call raises
 `LibraryMissing`.
@@ -29,6 +33,8 @@ from .grammar import (DfaSchemaGrammar, GbnfGrammarEngine, GbnfRule, GrammarCons
                       SchemaMismatch, StructuredOutputEngine, TokenBytes)
 from .decode import DecodeLoop, TokenEvent
 from .lm_head import LmHeadQ8_0, quantize_q8_1
+from .logprobs import TokenLogprobs
+from .lora import NO_ADAPTER, LoraAdapters
 from ._abi import (
     LibraryMissing,
     OxsError,
@@ -55,6 +61,9 @@ __all__ = [
     "TokenEvent",
     "LmHeadQ8_0",
     "quantize_q8_1",
+    "TokenLogprobs",
+    "LoraAdapters",
+    "NO_ADAPTER",
     "LibraryMissing",
     "OxsError",
     "load_library",

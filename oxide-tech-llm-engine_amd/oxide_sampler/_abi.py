@@ -35,6 +35,7 @@ OXS_MIROSTAT_V2 = 2
 
 OXS_DTYPE_F32 = 0
 OXS_DTYPE_BF16 = 1
+OXS_DTYPE_F16 = 2  # adapter weights only
 
 OXS_FLAG_RECORD_HISTORY = 1
 OXS_FLAG_SHARED_CONFIG = 2
@@ -76,9 +77,21 @@ EXPORTED_SYMBOLS = (
     "oxs_q8_0_packed_bytes",
     "oxs_pack_q8_0",
     "oxs_mmvq_q8_0",
+    "oxs_logprobs_workspace_bytes",
+    "oxs_token_logprobs",
+    "oxs_lora_table_bytes",
+    "oxs_lora_load",
+    "oxs_lora_workspace_bytes",
+    "oxs_lora_add",
 )
 
 OXS_DFA_ERROR_STATE = 0xFFFFFFFF
+
+OXS_LOGPROBS_MAX_TOP = 32
+OXS_LOGPROBS_MAX_TOKENS = 64
+
+OXS_LORA_MAX_RANK = 256
+OXS_LORA_NONE = 0xFFFFFFFF
 
 
 class OxsSamplingConfig(ctypes.Structure):
@@ -189,6 +202,62 @@ class OxsDecodeIo(ctypes.Structure):
     ]
 
 
+class OxsLogprobs(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_uint32),
+        ("vocab", ctypes.c_uint32),
+        ("logits_dtype", ctypes.c_int32),
+        ("tokens_per_row", ctypes.c_uint32),
+        ("logits_ld", ctypes.c_int64),
+        ("logits", ctypes.c_void_p),
+        ("tokens", ctypes.c_void_p),
+        ("tokens_ld", ctypes.c_int64),
+        ("allowed_mask", ctypes.c_void_p),
+        ("mask_ld", ctypes.c_int64),
+        ("temperatures", ctypes.c_void_p),
+        ("logit_softcap", ctypes.c_float),
+        ("top_n", ctypes.c_uint32),
+        ("out_logprobs", ctypes.c_void_p),
+        ("out_ranks", ctypes.c_void_p),
+        ("out_logsumexp", ctypes.c_void_p),
+        ("out_entropy", ctypes.c_void_p),
+        ("out_top_ids", ctypes.c_void_p),
+        ("out_top_logprobs", ctypes.c_void_p),
+        ("out_status", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class OxsLoraTable(ctypes.Structure):
+    _fields_ = [
+        ("m", ctypes.c_uint32),
+        ("k", ctypes.c_uint32),
+        ("max_adapters", ctypes.c_uint32),
+        ("max_rank", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        ("a", ctypes.c_void_p),
+        ("b", ctypes.c_void_p),
+        ("ranks", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+    ]
+
+
+class OxsLoraBatch(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_uint32),
+        ("x_dtype", ctypes.c_int32),
+        ("y_dtype", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("x_ld", ctypes.c_int64),
+        ("y", ctypes.c_void_p),
+        ("y_ld", ctypes.c_int64),
+        ("adapters", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
 _lib = None
 
 
@@ -271,6 +340,20 @@ def load_library(path: os.PathLike | str | None = None) -> ctypes.CDLL:
     lib.oxs_mmvq_q8_0.restype = ctypes.c_int
     lib.oxs_mmvq_q8_0.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32,
                                   ctypes.c_uint32, ctypes.c_uint32, ctypes.c_void_p]
+    lib.oxs_logprobs_workspace_bytes.restype = ctypes.c_size_t
+    lib.oxs_logprobs_workspace_bytes.argtypes = []
+    lib.oxs_token_logprobs.restype = ctypes.c_int
+    lib.oxs_token_logprobs.argtypes = [ctypes.POINTER(OxsLogprobs), ctypes.c_void_p]
+    lib.oxs_lora_table_bytes.restype = ctypes.c_int
+    lib.oxs_lora_table_bytes.argtypes = [ctypes.POINTER(OxsLoraTable), ctypes.POINTER(ctypes.c_size_t),
+                                         ctypes.POINTER(ctypes.c_size_t)]
+    lib.oxs_lora_load.restype = ctypes.c_int
+    lib.oxs_lora_load.argtypes = [ctypes.POINTER(OxsLoraTable), ctypes.c_uint32, ctypes.c_void_p, ctypes.c_int64,
+                                  ctypes.c_void_p, ctypes.c_int64, ctypes.c_uint32, ctypes.c_float, ctypes.c_void_p]
+    lib.oxs_lora_workspace_bytes.restype = ctypes.c_size_t
+    lib.oxs_lora_workspace_bytes.argtypes = [ctypes.POINTER(OxsLoraTable), ctypes.c_uint32]
+    lib.oxs_lora_add.restype = ctypes.c_int
+    lib.oxs_lora_add.argtypes = [ctypes.POINTER(OxsLoraTable), ctypes.POINTER(OxsLoraBatch), ctypes.c_void_p]
     if lib.oxs_abi_version() != OXS_ABI_VERSION:
         raise RuntimeError(f"liboxide_sampler ABI {lib.oxs_abi_version()} != {OXS_ABI_VERSION}")
     if path is None:

@@ -20,6 +20,12 @@ per-token bookkeeping stays on the host, as in the reference (:986-1030):
 stop tokens, the DFA state walk, accepting states and max_tokens. It is a few
 comparisons per sequence.
 
+With `top_logprobs` the step also computes, on the same stream, the log
+probability, rank and `top_logprobs` alternatives of every slot's token in the
+distribution of its logits (under the mask, before penalties and temperature),
+into the device tensors of `DecodeLoop.logprobs` (read them on the step's
+stream: the tokens reach the host before them).
+
 The step can be captured once in a HIP graph (`capture`) and replayed, since
 it issues only kernels.
 """
@@ -36,6 +42,7 @@ from . import _abi
 from ._abi import OxsDecodeIo, check
 from .engine import BatchSampler, SamplerState, SamplingConfig, _torch
 from .grammar import DFA_ERROR_STATE, DfaSchemaGrammar, SchemaMismatch
+from .logprobs import TokenLogprobs
 
 # Stop tokens without a tokenizer (continuous_batching.rs:990-1000).
 STOP_TOKENS = frozenset((0, 2, 128_001, 128_008, 128_009, 151_643, 151_645))
@@ -102,7 +109,9 @@ class DecodeLoop:
 
     def __init__(self, max_slots: int, vocab: int, history_cap: int = 4096, max_top_k: int = 256,
                  device: int = 0, token_bytes: Optional[Callable[[int], bytes]] = None,
-                 is_stop_token: Optional[Callable[[int], bool]] = None):
+                 is_stop_token: Optional[Callable[[int], bool]] = None, top_logprobs: Optional[int] = None):
+        if top_logprobs is not None and not 0 <= top_logprobs <= _abi.OXS_LOGPROBS_MAX_TOP:
+            raise ValueError(f"top_logprobs {top_logprobs} outside 0..{_abi.OXS_LOGPROBS_MAX_TOP}")
         t = _torch()
         self.torch = t
         self.sampler = BatchSampler(max_slots, vocab, max_top_k, device)
@@ -131,6 +140,17 @@ class DecodeLoop:
         self._slots = np.frombuffer((ctypes.c_uint64 * S).from_address(self._host), dtype=np.uint64)
         self.io = OxsDecodeIo(self.current_token.data_ptr(), self.current_position.data_ptr(),
                               self.generated_count.data_ptr(), self._host)
+        # log probabilities of each step's tokens, overwritten by every launch
+        self.top_logprobs = int(top_logprobs or 0)
+        self._logprobs: Optional[TokenLogprobs] = None
+        self.logprobs: Optional[dict] = None
+        if top_logprobs is not None:
+            self._logprobs = TokenLogprobs(device)
+            self.logprobs = {k: t.zeros(S, dtype=t.float32, device=dev) for k in ("logprobs", "logsumexp", "entropy")}
+            self.logprobs |= {k: t.zeros(S, dtype=t.int32, device=dev) for k in ("ranks", "status")}
+            if self.top_logprobs:
+                self.logprobs["top_ids"] = t.zeros(S, self.top_logprobs, dtype=t.int32, device=dev)
+                self.logprobs["top_logprobs"] = t.zeros(S, self.top_logprobs, dtype=t.float32, device=dev)
         self.launched = 0  # steps launched; every step covers every slot
         self._tokens = np.zeros(S, np.uint32)
         self.active: Dict[int, Sequence] = {}
@@ -190,9 +210,15 @@ class DecodeLoop:
     def _launch(self, logits, mask=None, stream=None) -> None:
         if tuple(logits.shape) != (self.max_slots, self.vocab):
             raise ValueError(f"logits must be [{self.max_slots}, {self.vocab}]")
+        call = None
+        if self._logprobs is not None:  # described first: what it refuses is refused before the step runs
+            call, _ = self._logprobs.descriptor(logits, self.out["tokens"], top=self.top_logprobs, mask=mask,
+                                                out=self.logprobs)
         self.sampler.sample(logits, self.configs, mask=mask, history=self.history, history_len=self.history_len,
                             history_cap=self.history_cap, record=True, rng_state=self.rng_state,
                             mirostat_mu=self.mirostat_mu, stream=stream, decode=self.io, out=self.out)
+        if call is not None:
+            self._logprobs.launch(call, stream)
 
     def launch(self, logits, mask=None, stream=None) -> int:
         """Queues one decode step over every slot; returns its step number."""

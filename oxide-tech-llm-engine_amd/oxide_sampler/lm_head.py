@@ -82,21 +82,32 @@ class LmHeadQ8_0:
                                 ctypes.c_void_p(self.packed.data_ptr()), _stream(t, dev, None)), "oxs_pack_q8_0")
         t.cuda.current_stream(dev).synchronize()  # src is freed on return
 
-    def project(self, x_q8_1, out=None, stream=None):
-        """launch_cuda_mmvq_q8_0: q8_1 activations (uint8 device tensor [batch, k / 32 * 36]) -> float32 [batch, m]."""
+    def project(self, x_q8_1, out=None, stream=None, adapters=None, x=None, row_adapters=None):
+        """launch_cuda_mmvq_q8_0: q8_1 activations (uint8 device tensor [batch, k / 32 * 36]) -> float32 [batch, m].
+
+        With `adapters` (a LoraAdapters over this head's m and k), each row's
+        adapter is added to that: `x` holds the activations before their
+        quantization ([batch, k]) and `row_adapters` each row's slot."""
         t = self.torch
         row_bytes = self.k // 32 * Q8_1_BYTES
         if x_q8_1.dtype != t.uint8 or not x_q8_1.is_cuda or x_q8_1.dim() != 2 or x_q8_1.shape[1] != row_bytes:
             raise ValueError(f"x_q8_1 must be a uint8 device tensor [batch, {row_bytes}]")
         if not x_q8_1.is_contiguous():
             raise ValueError("x_q8_1 must be contiguous")
-        x = x_q8_1
-        batch = x.shape[0]
+        xq = x_q8_1
+        batch = xq.shape[0]
+        if adapters is not None and (adapters.m, adapters.k) != (self.m, self.k):
+            raise ValueError(f"the adapters are for a head of {adapters.m} x {adapters.k}, not {self.m} x {self.k}")
+        if (adapters is None) != (x is None) or (adapters is None) != (row_adapters is None):
+            raise ValueError("adapters, x and row_adapters go together")
         if out is None:
-            out = t.empty(batch, self.m, dtype=t.float32, device=x.device)
+            out = t.empty(batch, self.m, dtype=t.float32, device=xq.device)
         elif tuple(out.shape) != (batch, self.m) or out.dtype != t.float32 or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous float32 tensor [{batch}, {self.m}]")
+        add = adapters.descriptor(out, x, row_adapters) if adapters is not None else None
         check(self.lib.oxs_mmvq_q8_0(ctypes.c_void_p(out.data_ptr()), ctypes.c_void_p(self.packed.data_ptr()),
-                                     ctypes.c_void_p(x.data_ptr()), self.m, self.k, batch,
-                                     _stream(t, x.device, stream)), "oxs_mmvq_q8_0")
+                                     ctypes.c_void_p(xq.data_ptr()), self.m, self.k, batch,
+                                     _stream(t, xq.device, stream)), "oxs_mmvq_q8_0")
+        if add is not None:
+            adapters.launch(add, stream)
         return out
