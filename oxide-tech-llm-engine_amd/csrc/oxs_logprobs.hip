@@ -4,10 +4,12 @@
 // With z the (softcapped, scaled) logits of a row's present tokens and m the
 // largest, one pass keeps m, s = sum e^(z - m) and t = sum (z - m) e^(z - m):
 //   lse = m + ln s,  log p_i = (z_i - m) - ln s,  H = ln s - t / s.
-// H's two terms are both >= 0, so nothing cancels.
+// H's two terms are both >= 0, so nothing cancels. Differences to m are taken
+// before the scaling, so large logits lose nothing either.
 //
-// One workgroup per row; the alternatives are found one after the other, each
-// by a pass for the largest key below the last.
+// rows_kernel: a workgroup reads a part of a row in tiles that stay in
+// registers; each thread keeps its own m, s and t. merge_kernel: a wavefront
+// joins the parts of a row where it was split over workgroups (few rows).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -17,15 +19,115 @@
 namespace oxs_lp {
 
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
 constexpr uint32_t kNoToken = 0xffffffffu;
-// e^-200 is 0 in 32 bits: a difference below this (or NaN, of two infinities) adds nothing
-constexpr float kFloor = -200.0f;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.693147180559945309417f;
+// 2^-256 is 0 in 32 bits: a difference below this (or NaN, of two infinities) adds nothing
+constexpr float kFloor = -256.0f;
+constexpr uint32_t kMaxSplits = 64;      // parts of a row
+constexpr uint32_t kMaxParts = 4096;     // rows * parts of a call that splits its rows
+constexpr uint32_t kMergeKeys = 20 * 64; // parts * top_n of a split row
+constexpr uint32_t kRoom = OXS_LOGPROBS_MAX_TOP + 512;  // candidates of a wavefront: those kept, and 64 lanes' next 8
 
 struct Params {
   oxs_logprobs b;
+  uint32_t splits;  // workgroups per row
+  uint32_t tiles;   // tiles per workgroup
+  // a split row's parts, in the workspace: [row * splits + part]
+  float4* stats;    // m (raw logit), s, t
+  uint64_t* keys;   // [top_n] the part's largest keys, in order, 0 past the last
+  uint32_t* counts; // [tokens_per_row] tokens of the part in front of each given token
 };
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+
+// Orders tokens: a larger logit first, then the lower id (+0.0 for both zeros).
+__device__ __forceinline__ uint32_t order_of(float l) {
+  const uint32_t u = __float_as_uint(l + 0.0f);
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float order_value(uint32_t o) {
+  return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o);
+}
+__device__ __forceinline__ uint64_t key_of(float l, uint32_t i) { return ((uint64_t)order_of(l) << 32) | (uint32_t)~i; }
+__device__ __forceinline__ float key_value(uint64_t k) { return order_value((uint32_t)(k >> 32)); }
+__device__ __forceinline__ uint32_t key_id(uint64_t k) { return ~(uint32_t)k; }
+
+constexpr uint32_t kOrderNegInf = 0x007fffffu;  // order_of(-inf)
+constexpr uint32_t kOrderZero = 0x80000000u;    // order_of(0)
+
+// The largest float below every l with order_of(l) >= o (the zeros are one value).
+__device__ __forceinline__ float just_below(uint32_t o) {
+  return o <= kOrderNegInf ? neg_inf() : order_value(o == kOrderZero ? o - 2u : o - 1u);
+}
+
+// ---------------------------------------------------------------- wavefront reductions (result in every lane)
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp(uint32_t other, uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)other, (int)x, CTRL, ROWS, 0xf, false);
+}
+template <class F>
+__device__ __forceinline__ uint32_t wave_reduce(uint32_t x, uint32_t identity, F f) {
+  x = f(x, dpp<0x111, 0xf>(identity, x));  // lanes 1, 2, 4, 8 below in the row of 16
+  x = f(x, dpp<0x112, 0xf>(identity, x));
+  x = f(x, dpp<0x114, 0xf>(identity, x));
+  x = f(x, dpp<0x118, 0xf>(identity, x));
+  x = f(x, dpp<0x142, 0xa>(identity, x));  // the row before, into rows 1 and 3
+  x = f(x, dpp<0x143, 0xc>(identity, x));  // lane 31, into rows 2 and 3
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+__device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
+  return wave_reduce(x, 0u, [](uint32_t a, uint32_t b) { return a + b; });
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  return __uint_as_float(wave_reduce(__float_as_uint(x), 0u, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  return __uint_as_float(wave_reduce(__float_as_uint(x), __float_as_uint(neg_inf()), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+
+// Orders a wavefront's accesses to LDS across its lanes.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// cap tanh(l / cap), to about 3 units in the last place: (1 - e) / (1 + e) with
+// e = e^(-2|x|), which cancels near 0, and the series up to x^9 below 1/4
+// (the next term is 0.009 x^10 <= 2^-26 of the value there).
+__device__ __forceinline__ float softcap_of(float l, float cap, float inv_cap) {
+  const float x = l * inv_cap, a = fabsf(x);
+  const float e = exp2_fast(a * (-2.0f * kLog2e));
+  const float far = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
+  const float w = a * a;
+  float p = __builtin_fmaf(w, 62.0f / 2835.0f, -17.0f / 315.0f);
+  p = __builtin_fmaf(w, p, 2.0f / 15.0f);
+  p = __builtin_fmaf(w, p, -1.0f / 3.0f);
+  const float near = __builtin_fmaf(a * w, p, a);
+  return cap * __builtin_copysignf(a < 0.25f ? near : far, x);
+}
+
+template <bool CAP>
+__device__ __forceinline__ float capped(float l, float cap, float inv_cap) {
+  if constexpr (CAP) return softcap_of(l, cap, inv_cap);
+  return l;
+}
+
+// 1 / T of a row, as the decode step takes it: greedy rows stay as they are.
+__device__ __forceinline__ float inverse_temperature(const oxs_logprobs& b, uint32_t row) {
+  if (!b.temperatures) return 1.0f;
+  const float t = b.temperatures[row];
+  return t > 1e-6f ? 1.0f / t : 1.0f;
+}
 
 // The logit of token i, -inf when it is not present.
 template <int DT>
@@ -43,129 +145,470 @@ __device__ __forceinline__ float present_logit(const oxs_logprobs& b, uint32_t r
   return l;
 }
 
-// Orders tokens: a larger logit first, then the lower id (+0.0 for both zeros).
-__device__ __forceinline__ uint64_t key_of(float l, uint32_t i) {
-  const uint32_t u = __float_as_uint(l + 0.0f);
-  const uint32_t o = (u & 0x80000000u) ? ~u : u | 0x80000000u;
-  return ((uint64_t)o << 32) | (uint32_t)~i;
-}
-__device__ __forceinline__ float key_value(uint64_t k) {
-  const uint32_t o = (uint32_t)(k >> 32);
-  return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o);
-}
-__device__ __forceinline__ uint32_t key_id(uint64_t k) { return ~(uint32_t)k; }
-
-__device__ __forceinline__ float softcap(float l, float cap) { return cap > 0.0f ? cap * tanhf(l / cap) : l; }
-
-template <int DT>
-__global__ __launch_bounds__(kThreads) void row_kernel(Params p) {
-  const oxs_logprobs& b = p.b;
-  const uint32_t row = blockIdx.x, tid = threadIdx.x;
-  __shared__ float s_m[kThreads], s_s[kThreads], s_t[kThreads];
-  __shared__ uint64_t s_key[kThreads];
-  __shared__ float s_tok[OXS_LOGPROBS_MAX_TOKENS];
-  __shared__ uint32_t s_rank[OXS_LOGPROBS_MAX_TOKENS];
-  float inv = 1.0f;
-  if (b.temperatures) {
-    const float t = b.temperatures[row];
-    if (t > 1e-6f) inv = 1.0f / t;
+// What a row's outputs follow from.
+struct Row {
+  float m, s, t;  // the largest raw logit; s and t relative to its z
+  float cap, inv_cap, inv;
+  float y_m, ln_s;
+  bool empty, over;
+  __device__ __forceinline__ Row(const oxs_logprobs& b, float inv_, float m_, float s_, float t_)
+      : m(m_), s(s_), t(t_), cap(b.logit_softcap), inv(inv_) {
+    inv_cap = 1.0f / cap;
+    empty = m == neg_inf();
+    y_m = y_of(m);
+    over = y_m == __builtin_inff();
+    ln_s = empty ? 0.0f : logf(s);
   }
-  for (uint32_t j = tid; j < b.tokens_per_row; j += kThreads) {
-    s_tok[j] = present_logit<DT>(b, row, b.tokens[(size_t)row * (size_t)b.tokens_ld + j]);
-    s_rank[j] = 0;
+  __device__ __forceinline__ float y_of(float l) const { return cap > 0.0f ? softcap_of(l, cap, inv_cap) : l; }
+  __device__ __forceinline__ float logprob(float l) const {  // of a raw logit
+    if (l == neg_inf()) return l;
+    const float y = y_of(l);
+    if (over) return y == y_m ? __builtin_nanf("") : neg_inf();
+    return (y - y_m) * inv - ln_s;
   }
-  __syncthreads();
-  // z relative to the largest so far, before the temperature
-  float m = neg_inf(), s = 0.0f, t = 0.0f;
-  for (uint32_t i = tid; i < b.vocab; i += kThreads) {
-    const float l = present_logit<DT>(b, row, i);
-    if (l == neg_inf()) continue;
-    const float y = softcap(l, b.logit_softcap);
-    if (y > m) {
-      const float d = fmaxf((m - y) * inv, kFloor);
-      const float f = expf(d);
-      t = f * (t + d * s);
-      s = f * s;
-      m = y;
-    }
-    const float q = fmaxf((y - m) * inv, kFloor), e = expf(q);
-    s += e;
-    t += q * e;
-    for (uint32_t j = 0; j < b.tokens_per_row; ++j) {
-      const uint32_t id = b.tokens[(size_t)row * (size_t)b.tokens_ld + j];
-      if (l > s_tok[j] || (l == s_tok[j] && i < id)) atomicAdd(&s_rank[j], 1u);
-    }
-  }
-  s_m[tid] = m;
-  s_s[tid] = s;
-  s_t[tid] = t;
-  __syncthreads();
-  for (int o = kThreads / 2; o > 0; o >>= 1) {
-    if (tid < (uint32_t)o) {
-      const float ma = s_m[tid], mb = s_m[tid + o], mm = fmaxf(ma, mb);
-      if (mm != neg_inf()) {
-        const float da = fmaxf((ma - mm) * inv, kFloor), db = fmaxf((mb - mm) * inv, kFloor);
-        const float fa = expf(da), fb = expf(db);
-        const float ta = fa * (s_t[tid] + da * s_s[tid]), tb = fb * (s_t[tid + o] + db * s_s[tid + o]);
-        s_s[tid] = fa * s_s[tid] + fb * s_s[tid + o];
-        s_t[tid] = ta + tb;
-        s_m[tid] = mm;
-      }
-    }
-    __syncthreads();
-  }
-  m = s_m[0];
-  s = s_s[0];
-  t = s_t[0];
-  const bool empty = m == neg_inf(), over = m == __builtin_inff();
-  const float ln_s = empty ? 0.0f : logf(s);
-  const auto logprob = [&](float l) {  // of a raw logit
-    if (l == neg_inf()) return neg_inf();
-    const float y = softcap(l, b.logit_softcap);
-    if (over) return y == m ? __builtin_nanf("") : neg_inf();
-    return (y - m) * inv - ln_s;
-  };
-  if (tid == 0) {
-    if (b.out_logsumexp) b.out_logsumexp[row] = empty || over ? m : m * inv + ln_s;
-    if (b.out_entropy) b.out_entropy[row] = empty ? 0.0f : over ? __builtin_nanf("") : ln_s - t / s;
+  __device__ __forceinline__ void write(const oxs_logprobs& b, uint32_t row) const {
+    if (b.out_logsumexp) b.out_logsumexp[row] = empty ? m : over ? y_m : y_m * inv + ln_s;
+    if (b.out_entropy) b.out_entropy[row] = empty ? 0.0f : over ? __builtin_nanf("") : ln_s - kLn2 * (t / s);
     if (b.out_status) b.out_status[row] = empty ? OXS_ROW_EMPTY : OXS_ROW_OK;
   }
-  for (uint32_t j = tid; j < b.tokens_per_row; j += kThreads) {
+  // given token j, with logit l and `before` tokens in front of it
+  __device__ __forceinline__ void write_token(const oxs_logprobs& b, uint32_t row, uint32_t j, float l,
+                                              uint32_t before) const {
     const size_t at = (size_t)row * b.tokens_per_row + j;
-    if (b.out_logprobs) b.out_logprobs[at] = logprob(s_tok[j]);
-    if (b.out_ranks) b.out_ranks[at] = s_tok[j] == neg_inf() ? 0u : s_rank[j] + 1u;
+    if (b.out_logprobs) b.out_logprobs[at] = logprob(l);
+    if (b.out_ranks) b.out_ranks[at] = l == neg_inf() ? 0u : before + 1u;
   }
-  uint64_t last = ~0ull;
-  for (uint32_t n = 0; n < b.top_n; ++n) {
+  __device__ __forceinline__ void write_top(const oxs_logprobs& b, uint32_t row, uint32_t n, uint64_t k) const {
+    const size_t at = (size_t)row * b.top_n + n;
+    if (b.out_top_ids) b.out_top_ids[at] = k ? key_id(k) : kNoToken;
+    if (b.out_top_logprobs) b.out_top_logprobs[at] = k ? logprob(key_value(k)) : neg_inf();
+  }
+};
+
+// The n largest of a wavefront's `count` <= kRoom keys in `keys` (LDS), in order, in its first places: n rounds of
+// taking the largest. Rare: many equal logits, or rows that rise towards their end.
+__device__ __forceinline__ uint32_t keep_largest(uint64_t* keys, uint32_t count, uint32_t n) {
+  const uint32_t lane = threadIdx.x & 63u;
+  constexpr int kPer = (kRoom + 63) / 64;
+  uint64_t mine[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) mine[i] = lane + 64u * i < count ? keys[lane + 64u * i] : 0;
+  wave_sync();
+  const uint32_t kept = min(n, count);
+  for (uint32_t r = 0; r < kept; ++r) {
     uint64_t best = 0;
-    for (uint32_t i = tid; i < b.vocab; i += kThreads) {
-      const float l = present_logit<DT>(b, row, i);
-      if (l == neg_inf()) continue;
-      const uint64_t k = key_of(l, i);
-      if (k < last && k > best) best = k;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) best = mine[i] > best ? mine[i] : best;
+    for (int o = 32; o > 0; o >>= 1) {
+      const uint64_t other = __shfl_xor((unsigned long long)best, o);
+      best = other > best ? other : best;
     }
-    s_key[tid] = best;
-    __syncthreads();
-    for (int o = kThreads / 2; o > 0; o >>= 1) {
-      if (tid < (uint32_t)o && s_key[tid + o] > s_key[tid]) s_key[tid] = s_key[tid + o];
-      __syncthreads();
-    }
-    best = s_key[0];
-    __syncthreads();
-    if (tid == 0) {
-      const size_t at = (size_t)row * b.top_n + n;
-      if (b.out_top_ids) b.out_top_ids[at] = best ? key_id(best) : kNoToken;
-      if (b.out_top_logprobs) b.out_top_logprobs[at] = best ? logprob(key_value(best)) : neg_inf();
-    }
-    last = best;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (mine[i] == best) mine[i] = 0;
+    if (lane == 0) keys[r] = best;
   }
+  wave_sync();
+  return kept;
+}
+
+// ---------------------------------------------------------------- the pass over the logits
+
+// G consecutive logits in one 16-byte load; a thread holds E of a tile as E / G groups that lie
+// kThreads * G apart. Rows that do not begin on 16 bytes are cut at the boundaries all the same: the
+// first and the last group of a row are then loaded one by one.
+template <int DT>
+constexpr int group_size() { return DT == OXS_DTYPE_F32 ? 4 : 8; }
+
+template <int DT, int E, bool MASK, bool CAP>
+__global__ __launch_bounds__(kThreads) void rows_kernel(Params p) {
+  constexpr int G = group_size<DT>(), NG = E / G;
+  constexpr uint32_t kTile = kThreads * E;
+  const oxs_logprobs& b = p.b;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+  const uint32_t row = blockIdx.x / p.splits, part = blockIdx.x - row * p.splits;
+  const uint32_t V = b.vocab, T = b.tokens_per_row, N = b.top_n;
+  __shared__ uint64_t s_keys[kWaves][kRoom];
+  __shared__ uint32_t s_order[2][kThreads];
+  __shared__ uint64_t s_list[kThreads];
+  __shared__ float s_m[kWaves], s_s[kWaves], s_t[kWaves];
+  __shared__ uint32_t s_count[kWaves];
+  __shared__ uint32_t s_before[kWaves][OXS_LOGPROBS_MAX_TOKENS];
+
+  const char* base = (const char*)b.logits + (size_t)row * (size_t)b.logits_ld * (DT == OXS_DTYPE_F32 ? 4 : 2);
+  // logits between the boundary before the row and its first one
+  const uint32_t skip = ((uint32_t)(uintptr_t)base & 15u) / (DT == OXS_DTYPE_F32 ? 4 : 2);
+  const uint32_t* mask = MASK ? b.allowed_mask + (size_t)row * (size_t)b.mask_ld : nullptr;
+  const float inv = inverse_temperature(b, row), c = inv * kLog2e;
+  const float cap = b.logit_softcap, inv_cap = CAP ? 1.0f / cap : 0.0f;
+
+  // lane j's given token
+  uint32_t want = kNoToken;
+  float want_l = neg_inf();
+  if (lane < T) want = b.tokens[(size_t)row * (size_t)b.tokens_ld + lane];
+
+  float m = neg_inf(), s = 0.0f, t = 0.0f;  // this thread's
+  float floor = neg_inf();                  // every alternative of the row is above it
+  float bound = neg_inf();                  // and those of this wavefront's tokens to come above this
+  uint32_t count = 0, round = 0;            // candidates of this wavefront; times the bound was raised
+  uint64_t* keys = s_keys[wave];
+  if (lane < T) s_before[wave][lane] = 0;
+
+  const uint32_t first = part * p.tiles;
+  const uint32_t total = (V + skip + kTile - 1u) / kTile;
+  const uint32_t last = min(first + p.tiles, total);
+  for (uint32_t tile = first; tile < last; ++tile) {
+    // element e of group g is token at + g * kThreads * G + e (negative before the row: none)
+    const int64_t at0 = (int64_t)tile * kTile + tid * G - (int64_t)skip;
+    const int32_t at = (int32_t)at0;  // V <= 2^30
+    float v[E];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const int32_t i = at + g * kThreads * G;
+      if (i >= 0 && i + G <= (int32_t)V) {
+        if constexpr (DT == OXS_DTYPE_F32) {
+          typedef float f4 __attribute__((ext_vector_type(4)));
+          const f4 x = __builtin_nontemporal_load((const f4*)(base + (int64_t)i * 4));
+#pragma unroll
+          for (int e = 0; e < G; ++e) v[g * G + e] = x[e];
+        } else {
+          typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+          const u4 x = __builtin_nontemporal_load((const u4*)(base + (int64_t)i * 2));
+#pragma unroll
+          for (int e = 0; e < G; ++e)
+            v[g * G + e] = __uint_as_float((e & 1) ? x[e >> 1] & 0xffff0000u : x[e >> 1] << 16);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < G; ++e) {
+          v[g * G + e] = neg_inf();
+          if (i + e >= 0 && i + e < (int32_t)V) {
+            if constexpr (DT == OXS_DTYPE_F32) v[g * G + e] = ((const float*)base)[i + e];
+            else v[g * G + e] = __uint_as_float((uint32_t)((const uint16_t*)base)[i + e] << 16);
+          }
+        }
+      }
+    }
+    if constexpr (MASK) {
+      const uint32_t words = (V + 31u) / 32u;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const int32_t i = max(at + g * kThreads * G, 0);  // (before the row: -inf already; its bits are those from 0 on)
+        const int32_t d = i - (at + g * kThreads * G);
+        const uint32_t w = min((uint32_t)i >> 5, words - 1u);
+        uint32_t bits = mask[w] >> (i & 31);
+        if ((i & 31) > 32 - G && w + 1u < words) bits |= mask[w + 1u] << (32 - (i & 31));
+        bits <<= d;
+#pragma unroll
+        for (int e = 0; e < G; ++e)
+          if (!((bits >> e) & 1u)) v[g * G + e] = neg_inf();
+      }
+    }
+    if (tile == first && lane < T) want_l = present_logit<DT>(b, row, want);
+
+    // the thread's largest (the maximum passes over quiet NaNs only)
+    float top = __builtin_canonicalizef(v[0]);
+#pragma unroll
+    for (int e = 1; e < E; ++e) top = fmaxf(top, v[e]);
+    const float old = m;
+    m = fmaxf(m, top);
+
+    if (N) {
+      // Raise the floor at the 1st, 2nd, 4th, ... and last tile: at least N logits so far are no less than
+      // the N-th largest of the 256 threads' maxima, so the rest cannot be alternatives.
+      const uint32_t n = tile - first + 1u;
+      if ((n & (n - 1u)) == 0u || tile + 1u == last) {
+        uint32_t* so = s_order[round & 1u];  // (a wavefront is at most one round ahead)
+        ++round;
+        so[tid] = order_of(m);
+        __syncthreads();
+        uint32_t o[kWaves];
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) o[w] = so[w * 64 + lane];
+        uint32_t lo = kOrderNegInf, hi = 0xffffffffu;  // N maxima are >= lo, fewer are >= hi
+        for (int step = 0; step < 32 && hi - lo > 1u; ++step) {
+          const uint32_t mid = lo + (hi - lo) / 2u;
+          uint32_t k = 0;
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) k += (uint32_t)__popcll(__ballot(o[w] >= mid));
+          if (k >= N) lo = mid;
+          else hi = mid;
+          if (k >= N && k <= N + 4u) break;
+        }
+        floor = fmaxf(floor, just_below(lo));
+        bound = fmaxf(bound, floor);
+      }
+      if (__ballot(top > bound)) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          float gm = v[g * G];
+#pragma unroll
+          for (int e = 1; e < G; ++e) gm = fmaxf(gm, v[g * G + e]);
+          if (!__ballot(gm > bound)) continue;
+          if (count + 64u * G > kRoom) {  // room for the whole group
+            count = keep_largest(keys, count, N);
+            // later tokens of this wavefront have larger ids: equal ones come after
+            if (count == N) bound = fmaxf(bound, key_value(keys[N - 1u]));
+          }
+#pragma unroll
+          for (int e = 0; e < G; ++e) {
+            const float x = v[g * G + e];
+            const uint64_t who = __ballot(x > bound);
+            if (who) {
+              if (x > bound)
+                keys[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32),
+                                                       __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u))] =
+                    key_of(x, (uint32_t)(at + g * kThreads * G + e));
+              count += (uint32_t)__popcll(who);
+            }
+          }
+        }
+      }
+    }
+
+    {  // s and t, relative to the thread's new maximum
+      const float y_m = capped<CAP>(m, cap, inv_cap);
+      const float d = fmaxf((capped<CAP>(old, cap, inv_cap) - y_m) * c, kFloor), f = exp2_fast(d);
+      float s0 = f * s, t0 = f * __builtin_fmaf(d, s, t), s1 = 0.0f, t1 = 0.0f;
+      if (old == neg_inf()) s0 = t0 = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float q0 = fmaxf((capped<CAP>(v[e], cap, inv_cap) - y_m) * c, kFloor);
+        const float q1 = fmaxf((capped<CAP>(v[e + 1], cap, inv_cap) - y_m) * c, kFloor);
+        float p0 = exp2_fast(q0), p1 = exp2_fast(q1);
+        if constexpr (CAP) {  // the cap of -inf is a value
+          p0 = v[e] == neg_inf() ? 0.0f : p0;
+          p1 = v[e + 1] == neg_inf() ? 0.0f : p1;
+        }
+        s0 += p0;
+        s1 += p1;
+        t0 = __builtin_fmaf(q0, p0, t0);
+        t1 = __builtin_fmaf(q1, p1, t1);
+      }
+      s = s0 + s1;
+      t = t0 + t1;
+    }
+
+    // tokens in front of the given ones
+    for (uint32_t j = 0; j < T; ++j) {
+      const float l = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(want_l), (int)j));
+      if (l == neg_inf()) continue;
+      const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)want, (int)j);
+      const uint64_t begin = (uint64_t)tile * kTile;  // of the tile, in tokens + skip
+      uint32_t k = 0;
+      if (begin + kTile <= (uint64_t)id + skip) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) k += v[e] >= l ? 1u : 0u;
+      } else if (begin > (uint64_t)id + skip) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) k += v[e] > l ? 1u : 0u;
+      } else {
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int e = 0; e < G; ++e) {
+            const bool lower = at + g * kThreads * G + e < (int32_t)id;
+            const float x = v[g * G + e];
+            k += (x > l || (x == l && lower)) ? 1u : 0u;
+          }
+      }
+      k = wave_sum(k);
+      if (lane == j) s_before[wave][j] += k;
+    }
+  }
+
+  // the workgroup's sums
+  {
+    const float wm = wave_max(m), y_m = capped<CAP>(wm, cap, inv_cap);
+    const float d = fmaxf((capped<CAP>(m, cap, inv_cap) - y_m) * c, kFloor);
+    const float f = m == neg_inf() ? 0.0f : exp2_fast(d);
+    const float ws = wave_sum(f * s), wt = wave_sum(f * __builtin_fmaf(d, s, t));
+    if (lane == 0) {
+      s_m[wave] = wm;
+      s_s[wave] = ws;
+      s_t[wave] = wt;
+    }
+  }
+  if (N) {
+    // drop what the last floor leaves out, and keep at most 64 candidates per wavefront
+    uint32_t kept = 0;
+    for (uint32_t i0 = 0; i0 < count; i0 += 64u) {
+      const uint64_t k = i0 + lane < count ? keys[i0 + lane] : 0;
+      const bool in = k && key_value(k) > floor;
+      const uint64_t who = __ballot(in);
+      wave_sync();
+      if (in)
+        keys[kept + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u))] = k;
+      kept += (uint32_t)__popcll(who);
+    }
+    wave_sync();
+    count = kept > 64u ? keep_largest(keys, kept, N) : kept;
+    if (lane == 0) s_count[wave] = count;
+  }
+  __syncthreads();
+  float bm = s_m[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) bm = s_m[w] > bm ? s_m[w] : bm;
+  float bs = 0.0f, bt = 0.0f;
+  {
+    const float y_m = capped<CAP>(bm, cap, inv_cap);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float d = fmaxf((capped<CAP>(s_m[w], cap, inv_cap) - y_m) * c, kFloor);
+      const float f = s_m[w] == neg_inf() ? 0.0f : exp2_fast(d);
+      bs += f * s_s[w];
+      bt += f * __builtin_fmaf(d, s_s[w], s_t[w]);
+    }
+  }
+  uint32_t before_me = 0, all = 0;
+  if (N) {  // one list of the workgroup's candidates
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < (int)wave) before_me += s_count[w];
+      all += s_count[w];
+    }
+    if (lane < count) s_list[before_me + lane] = keys[lane];
+    __syncthreads();
+  }
+  uint32_t before = 0;  // of given token tid
+  if (tid < T)
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) before += s_before[w][tid];
+  uint64_t mine = 0;
+  uint32_t place = kNoToken;
+  if (tid < all) {
+    mine = s_list[tid];
+    place = 0;
+    for (uint32_t i = 0; i < all; ++i) place += s_list[i] > mine ? 1u : 0u;
+  }
+  if (p.splits > 1u) {
+    const size_t at = (size_t)row * p.splits + part;
+    if (tid == 0) p.stats[at] = make_float4(bm, bs, bt, 0.0f);
+    if (tid < T) p.counts[at * T + tid] = before;
+    if (place < N) p.keys[at * N + place] = mine;
+    if (tid >= all && tid < N) p.keys[at * N + tid] = 0;
+    return;
+  }
+  const Row r(b, inv, bm, bs, bt);
+  if (tid == 0) r.write(b, row);
+  if (tid < T) r.write_token(b, row, tid, want_l, before);  // (T <= 64: the first wavefront)
+  if (place < N) r.write_top(b, row, place, mine);
+  if (tid >= all && tid < N) r.write_top(b, row, tid, 0);
+}
+
+// One wavefront joins the parts of a row. The alternatives are the keys no less than a bound that is
+// found by halving the range of keys until N to N + 4 of them are above it.
+template <int DT, bool CAP, int PER>
+__global__ __launch_bounds__(64) void merge_kernel(Params p) {
+  const oxs_logprobs& b = p.b;
+  const uint32_t row = blockIdx.x, lane = threadIdx.x;
+  const uint32_t S = p.splits, T = b.tokens_per_row, N = b.top_n;
+  __shared__ uint64_t s_list[64];
+  const size_t at = (size_t)row * S;
+  float4 st = make_float4(neg_inf(), 0.0f, 0.0f, 0.0f);
+  if (lane < S) st = p.stats[at + lane];
+  uint64_t k[PER];
+  if (N) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) k[i] = lane + 64u * i < S * N ? p.keys[at * N + lane + 64u * i] : 0;
+  }
+  uint32_t want = kNoToken;
+  float want_l = neg_inf();
+  if (lane < T) {
+    want = b.tokens[(size_t)row * (size_t)b.tokens_ld + lane];
+    want_l = present_logit<DT>(b, row, want);
+  }
+  const float inv = inverse_temperature(b, row), c = inv * kLog2e;
+  const float cap = b.logit_softcap, inv_cap = CAP ? 1.0f / cap : 0.0f;
+  const float m = wave_max(st.x);
+  const float d = fmaxf((capped<CAP>(st.x, cap, inv_cap) - capped<CAP>(m, cap, inv_cap)) * c, kFloor);
+  const float f = st.x == neg_inf() ? 0.0f : exp2_fast(d);
+  const Row r(b, inv, m, wave_sum(f * st.y), wave_sum(f * __builtin_fmaf(d, st.y, st.z)));
+  if (lane == 0) r.write(b, row);
+  uint32_t before = 0;
+  for (uint32_t j = 0; j < T; ++j) {
+    const uint32_t n = wave_sum(lane < S ? p.counts[(at + lane) * T + j] : 0u);
+    if (lane == j) before = n;
+  }
+  if (lane < T) r.write_token(b, row, lane, want_l, before);
+  if (!N) return;
+  uint64_t lo = 1, hi = ~0ull;  // keys >= lo are enough (or all there are); fewer than N are >= hi
+  uint32_t n = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) n += (uint32_t)__popcll(__ballot(k[i] >= lo));
+  for (int step = 0; step < 64 && n > N + 4u; ++step) {
+    const uint64_t mid = lo + (hi - lo) / 2u;
+    uint32_t some = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) some += (uint32_t)__popcll(__ballot(k[i] >= mid));
+    if (some >= N) {
+      lo = mid;
+      n = some;
+    } else {
+      hi = mid;
+    }
+  }
+  uint32_t all = 0;  // n of them: at most N + 4 <= 64, as keys differ
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const bool in = k[i] >= lo;
+    const uint64_t who = __ballot(in);
+    const uint32_t to =
+        all + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
+    if (in && to < 64u) s_list[to] = k[i];
+    all += (uint32_t)__popcll(who);
+  }
+  all = min(all, 64u);
+  __syncthreads();
+  uint32_t place = kNoToken;
+  uint64_t mine = 0;
+  if (lane < all) {
+    mine = s_list[lane];
+    place = 0;
+    for (uint32_t i = 0; i < all; ++i) place += s_list[i] > mine ? 1u : 0u;
+  }
+  if (place < N) r.write_top(b, row, place, mine);
+  if (lane >= all && lane < N) r.write_top(b, row, lane, 0);
+}
+
+template <int DT, bool CAP>
+static void launch(Params& p, hipStream_t st) {
+  const oxs_logprobs& b = p.b;
+  // Tiles of 8192 logits (32 per thread), or of 2048 where those would leave CUs without a workgroup.
+  const auto tiles_of = [&](uint32_t tile) { return (b.vocab + 7u + tile - 1u) / tile; };
+  const bool small = (uint64_t)b.rows * tiles_of(kThreads * 32) < 256u;
+  const uint32_t tiles = tiles_of(kThreads * (small ? 8 : 32));
+  uint32_t splits = 1;
+  if (b.rows < 512u) {
+    splits = min(min(tiles, kMaxSplits), (1024u + b.rows - 1u) / b.rows);
+    if (b.top_n) splits = min(splits, kMergeKeys / b.top_n);
+  }
+  p.tiles = (tiles + splits - 1u) / splits;
+  p.splits = (tiles + p.tiles - 1u) / p.tiles;
+  const dim3 grid(b.rows * p.splits);
+  const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, p); };
+  if (b.allowed_mask) {
+    if (small) go(rows_kernel<DT, 8, true, CAP>);
+    else go(rows_kernel<DT, 32, true, CAP>);
+  } else {
+    if (small) go(rows_kernel<DT, 8, false, CAP>);
+    else go(rows_kernel<DT, 32, false, CAP>);
+  }
+  if (p.splits == 1u) return;
+  const auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(b.rows), dim3(64), 0, st, p); };
+  if (p.splits * b.top_n <= 5u * 64u) join(merge_kernel<DT, CAP, 5>);
+  else join(merge_kernel<DT, CAP, 20>);
 }
 
 }  // namespace oxs_lp
 
 static bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1u)) == 0; }
 
-extern "C" size_t oxs_logprobs_workspace_bytes(void) { return 16; }
+// stats, keys and counts of kMaxParts parts
+extern "C" size_t oxs_logprobs_workspace_bytes(void) {
+  return (size_t)oxs_lp::kMaxParts * (16u + 8u * OXS_LOGPROBS_MAX_TOP + 4u * OXS_LOGPROBS_MAX_TOKENS);
+}
 
 extern "C" int oxs_token_logprobs(const oxs_logprobs* lp, void* stream) {
   if (!lp) return OXS_ERR_INVALID_ARGUMENT;
@@ -187,11 +630,19 @@ extern "C" int oxs_token_logprobs(const oxs_logprobs* lp, void* stream) {
       !aligned(b.out_status, 4))
     return OXS_ERR_INVALID_ARGUMENT;
   if (b.workspace_bytes < oxs_logprobs_workspace_bytes()) return OXS_ERR_INVALID_ARGUMENT;
-  oxs_lp::Params p{b};
-  const auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(b.rows), dim3(oxs_lp::kThreads), 0, (hipStream_t)stream, p);
-  };
-  if (b.logits_dtype == OXS_DTYPE_F32) go(oxs_lp::row_kernel<OXS_DTYPE_F32>);
-  else go(oxs_lp::row_kernel<OXS_DTYPE_BF16>);
+  oxs_lp::Params p{};
+  p.b = b;
+  p.stats = (float4*)b.workspace;
+  p.keys = (uint64_t*)(p.stats + oxs_lp::kMaxParts);
+  p.counts = (uint32_t*)(p.keys + (size_t)oxs_lp::kMaxParts * OXS_LOGPROBS_MAX_TOP);
+  const bool cap = b.logit_softcap > 0.0f;
+  const hipStream_t st = (hipStream_t)stream;
+  if (b.logits_dtype == OXS_DTYPE_F32) {
+    if (cap) oxs_lp::launch<OXS_DTYPE_F32, true>(p, st);
+    else oxs_lp::launch<OXS_DTYPE_F32, false>(p, st);
+  } else {
+    if (cap) oxs_lp::launch<OXS_DTYPE_BF16, true>(p, st);
+    else oxs_lp::launch<OXS_DTYPE_BF16, false>(p, st);
+  }
   return hipGetLastError() == hipSuccess ? OXS_OK : OXS_ERR_HIP;
 }
