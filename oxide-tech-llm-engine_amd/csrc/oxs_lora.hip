@@ -1,8 +1,15 @@
 // oxs_lora.hip — low-rank adapters of many requests beside the projection
 // that they share: y_b += B_a (s_a A_a x_b) for the adapter a of each row b.
 //
-// Two launches: v_b = s_a A_a x_b into the workspace, then y_b += B_a v_b. A
-// wavefront sums one value of v; a thread owns one value of y.
+// shrink_kernel: v_b = s_a A_a x_b into the workspace. expand_kernel:
+// y_b += B_a v_b on the matrix cores, 32 rows x 64 or 128 outputs per
+// wavefront, for each adapter among the 32 rows in turn.
+//
+// The matrix cores take bf16. A float is the sum of three bf16 (each the
+// nearest to what is left of it: 2^-9 of it remains after one, 2^-18 after
+// two, nothing of its 24 bits after three), a half of two, so the products of
+// the parts in 32-bit sums give the product of the floats; of f32 weights'
+// nine products the three below 2^-26 of the whole are left out.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -12,35 +19,91 @@
 
 namespace oxs_lora {
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr uint32_t kRows = 32;        // rows of a matrix tile
+constexpr uint32_t kGroup = 128;      // outputs of a group in the table
+constexpr uint32_t kBlock = 16;       // ranks of a block: the depth of a matrix instruction
+constexpr uint32_t kPlanes = 3;       // bf16 parts of a value of v
+constexpr uint32_t kValueBytes = kPlanes * kBlock * 2;  // a row's values of a rank block: [part][16]
 
-template <int DT>
-__device__ __forceinline__ float load(const void* p, size_t i) {
-  if constexpr (DT == OXS_DTYPE_F32) return ((const float*)p)[i];
-  else if constexpr (DT == OXS_DTYPE_F16) return (float)((const _Float16*)p)[i];
-  else return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
+// Table, per slot:
+//   a  [ranks, a multiple of 16][k, rounded up to 8], zero past the adapter's
+//   b  [group of 128 outputs][rank block][half of the block][4][32] pieces of 8 ranks of one output, as a lane of a
+//      matrix instruction takes them: piece (t, n) belongs to output 4 n + t of the group. The half of a block that
+//      holds no rank is never read.
+__host__ __device__ __forceinline__ uint32_t rank_blocks(uint32_t rank) { return (rank + kBlock - 1u) / kBlock; }
+__host__ __device__ __forceinline__ uint32_t groups_of(uint32_t m) { return (m + kGroup - 1u) / kGroup; }
+__host__ __device__ __forceinline__ uint32_t padded_k(uint32_t k) { return (k + 7u) & ~7u; }
+__host__ __device__ __forceinline__ size_t a_elements(const oxs_lora_table& t) {
+  return (size_t)rank_blocks(t.max_rank) * kBlock * padded_k(t.k);
+}
+__host__ __device__ __forceinline__ size_t b_elements(const oxs_lora_table& t) {
+  return (size_t)groups_of(t.m) * rank_blocks(t.max_rank) * kBlock * kGroup;
 }
 
-// a value rounded to bf16, to the nearest, ties to even; NaN stays NaN
-__device__ __forceinline__ uint16_t to_bf16(float f) {
-  const uint32_t u = __float_as_uint(f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
+template <int DT>
+using Element = std::conditional_t<DT == OXS_DTYPE_F32, uint32_t, uint16_t>;
 
 template <int DT>
-__global__ __launch_bounds__(kThreads) void load_kernel(oxs_lora_table t, uint32_t slot, const void* a, int64_t a_ld,
-                                                        const void* b, int64_t b_ld, uint32_t rank, float scale) {
-  using E = std::conditional_t<DT == OXS_DTYPE_F32, uint32_t, uint16_t>;
-  const size_t na = (size_t)rank * t.k, nb = (size_t)rank * t.m;
+__device__ __forceinline__ float widen(uint32_t bits) {
+  if constexpr (DT == OXS_DTYPE_F32) return __uint_as_float(bits);
+  else if constexpr (DT == OXS_DTYPE_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+  else return __uint_as_float(bits << 16);
+}
+
+// Eight values from 16-byte aligned memory (two 16-byte loads for f32).
+template <int DT>
+struct Eight {
+  u32x4 q[DT == OXS_DTYPE_F32 ? 2 : 1];
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (DT == OXS_DTYPE_F32) return __uint_as_float(q[i / 4][i % 4]);
+    else if constexpr (DT == OXS_DTYPE_F16) return widen<DT>((q[0][i / 2] >> (16 * (i % 2))) & 0xffffu);
+    else return __uint_as_float(i % 2 ? q[0][i / 2] & 0xffff0000u : q[0][i / 2] << 16);
+  }
+};
+
+// Two floats as the nearest bf16 pair, and that pair widened again.
+__device__ __forceinline__ uint32_t narrow2(float x, float y) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x, y}, bf16x2));
+}
+__device__ __forceinline__ float low(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float high(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
+
+// ---------------------------------------------------------------- the table
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void load_kernel(oxs_lora_table t, uint32_t slot, const Element<DT>* a,
+                                                        int64_t a_ld, const Element<DT>* b, int64_t b_ld, uint32_t rank,
+                                                        float scale) {
+  const uint32_t blocks = rank_blocks(rank), kp = padded_k(t.k), all_blocks = rank_blocks(t.max_rank);
+  const size_t na = (size_t)blocks * kBlock * kp, nb = (size_t)groups_of(t.m) * blocks * kBlock * kGroup;
   const size_t step = (size_t)gridDim.x * kThreads;
-  E* ta = (E*)t.a + (size_t)slot * t.max_rank * t.k;
-  E* tb = (E*)t.b + (size_t)slot * t.max_rank * t.m;
+  Element<DT>* ta = (Element<DT>*)t.a + (size_t)slot * a_elements(t);
+  Element<DT>* tb = (Element<DT>*)t.b + (size_t)slot * b_elements(t);
   for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < na + nb; i += step) {
-    if (i < na) ta[i] = ((const E*)a)[(i / t.k) * (size_t)a_ld + i % t.k];
-    else {
+    if (i < na) {
+      const uint32_t r = (uint32_t)(i / kp), c = (uint32_t)(i % kp);
+      ta[i] = r < rank && c < t.k ? a[(size_t)r * (size_t)a_ld + c] : 0;
+    } else {
       const size_t j = i - na;
-      tb[(j / rank) * t.max_rank + j % rank] = ((const E*)b)[(j / rank) * (size_t)b_ld + j % rank];
+      // j counts [group][block][half][t][n][8 ranks] of the blocks that the adapter has
+      const uint32_t e = (uint32_t)(j & 7u), n = (uint32_t)(j >> 3) & 31u, tt = (uint32_t)(j >> 8) & 3u;
+      const uint32_t half = (uint32_t)(j >> 10) & 1u;
+      const size_t gb = j >> 11;
+      const uint32_t block = (uint32_t)(gb % blocks);
+      const size_t group = gb / blocks;
+      const uint32_t r = block * kBlock + half * 8u + e;
+      const size_t out = group * kGroup + 4u * n + tt;
+      tb[(group * all_blocks + block) * (kBlock * kGroup) + (j & 2047u)] =
+          r < rank && out < t.m ? b[out * (size_t)b_ld + r] : 0;
     }
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -49,34 +112,259 @@ __global__ __launch_bounds__(kThreads) void load_kernel(oxs_lora_table t, uint32
   }
 }
 
-template <int WT, int XT>
-__global__ __launch_bounds__(kThreads) void shrink_kernel(oxs_lora_table t, oxs_lora_batch b) {
-  const uint32_t row = blockIdx.x, r = blockIdx.y * (kThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63u;
-  const uint32_t a = b.adapters[row];
-  if (a >= t.max_adapters || r >= min(t.ranks[a], t.max_rank)) return;
-  const size_t w0 = ((size_t)a * t.max_rank + r) * t.k, x0 = (size_t)row * (size_t)b.x_ld;
-  float s = 0.0f;
-  for (uint32_t i = lane; i < t.k; i += 64) s = __builtin_fmaf(load<WT>(t.a, w0 + i), load<XT>(b.x, x0 + i), s);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if (lane == 0) ((float*)b.workspace)[(size_t)row * t.max_rank + r] = s * t.scales[a];
+// ---------------------------------------------------------------- v_b = s_a A_a x_b
+
+__device__ __forceinline__ uint32_t rank_of(const oxs_lora_table& t, uint32_t a) {
+  return a < t.max_adapters ? min(t.ranks[a], t.max_rank) : 0u;
 }
 
-template <int WT, int YT>
-__global__ __launch_bounds__(kThreads) void expand_kernel(oxs_lora_table t, oxs_lora_batch b) {
-  const uint32_t blocks = (t.m + kThreads - 1) / kThreads;
-  const uint32_t row = blockIdx.x / blocks, i = (blockIdx.x % blocks) * kThreads + threadIdx.x;
-  const uint32_t a = b.adapters[row];
-  if (a >= t.max_adapters || i >= t.m) return;
-  const uint32_t rank = min(t.ranks[a], t.max_rank);
-  if (rank == 0) return;
-  const float* v = (const float*)b.workspace + (size_t)row * t.max_rank;
-  const size_t w0 = ((size_t)a * t.m + i) * t.max_rank, at = (size_t)row * (size_t)b.y_ld + i;
-  float s = 0.0f;
-  for (uint32_t r = 0; r < rank; ++r) s = __builtin_fmaf(load<WT>(t.b, w0 + r), v[r], s);
-  const float y = load<YT>(b.y, at) + s;
-  if constexpr (YT == OXS_DTYPE_F32) ((float*)b.y)[at] = y;
-  else ((uint16_t*)b.y)[at] = to_bf16(y);
+// The parts of one value, for the matrix cores; an infinity or NaN has one part.
+__device__ __forceinline__ void store_value(void* workspace, uint32_t row, uint32_t all_blocks, uint32_t r, float v) {
+  uint16_t* to = (uint16_t*)workspace + ((size_t)row * all_blocks + r / kBlock) * (kValueBytes / 2) + r % kBlock;
+  const uint32_t p0 = narrow2(v, 0.0f) & 0xffffu;
+  const bool finite = fabsf(low(p0)) < __builtin_inff();
+  const float v1 = finite ? v - low(p0) : 0.0f;
+  const uint32_t p1 = narrow2(v1, 0.0f) & 0xffffu;
+  const uint32_t p2 = narrow2(v1 - low(p1), 0.0f) & 0xffffu;
+  to[0] = (uint16_t)p0;
+  to[kBlock] = (uint16_t)p1;
+  to[2 * kBlock] = (uint16_t)p2;
+}
+
+template <int DT>
+__device__ __forceinline__ Eight<DT> load_eight(const Element<DT>* p) {
+  Eight<DT> e;
+  e.q[0] = *(const u32x4*)p;
+  if constexpr (DT == OXS_DTYPE_F32) e.q[1] = *(const u32x4*)(p + 4);
+  return e;
+}
+
+// One wavefront per (row, PER ranks): its lanes take eight values of x at a time.
+template <int WT, int XT, int PER>
+__global__ __launch_bounds__(kThreads) void shrink_kernel(oxs_lora_table t, oxs_lora_batch b, uint32_t vec) {
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t row = blockIdx.x, r0 = (blockIdx.y * kWaves + wave) * PER;
+  const uint32_t a = b.adapters[row], rank = rank_of(t, a), all_blocks = rank_blocks(t.max_rank);
+  if (r0 >= rank_blocks(rank) * kBlock) return;
+  const uint32_t kp = padded_k(t.k);
+  const Element<WT>* w = (const Element<WT>*)t.a + (size_t)a * a_elements(t) + (size_t)r0 * kp;
+  const Element<XT>* x = (const Element<XT>*)b.x + (size_t)row * (size_t)b.x_ld;
+  float s[PER];
+#pragma unroll
+  for (int p = 0; p < PER; ++p) s[p] = 0.0f;
+#pragma unroll 4
+  for (uint32_t i = lane * 8u; i < t.k; i += 512u) {
+    float xv[8];
+    if (vec && i + 8u <= t.k) {
+      const Eight<XT> e = load_eight<XT>(x + i);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) xv[j] = e[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) xv[j] = i + j < t.k ? widen<XT>(x[i + j]) : 0.0f;
+    }
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const Eight<WT> e = load_eight<WT>(w + (size_t)p * kp + i);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[p] = __builtin_fmaf(e[j], xv[j], s[p]);
+    }
+  }
+  const float scale = t.scales[a];
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    float v = s[p];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    // ranks past the adapter's, up to the block's end, are zero
+    if (lane == 0) store_value(b.workspace, row, all_blocks, r0 + p, r0 + p < rank ? v * scale : 0.0f);
+  }
+}
+
+// ---------------------------------------------------------------- y_b += B_a v_b
+
+// Row i of the 32 x 32 output held in register r of a lane in half g.
+__device__ __forceinline__ uint32_t out_row(uint32_t r, uint32_t g) { return 8u * (r >> 2) + 4u * g + (r & 3u); }
+
+// The bf16 parts of eight weights.
+template <int WT>
+struct Parts {
+  static constexpr int N = WT == OXS_DTYPE_F32 ? 3 : WT == OXS_DTYPE_F16 ? 2 : 1;
+  bf16x8 p[N];
+  __device__ __forceinline__ Parts(const Eight<WT>& w) {
+    if constexpr (WT == OXS_DTYPE_BF16) {
+      p[0] = __builtin_bit_cast(bf16x8, w.q[0]);
+    } else {
+      u32x4 q[N];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = w[2 * i], y = w[2 * i + 1];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          q[n][i] = narrow2(x, y);
+          x -= low(q[n][i]);
+          y -= high(q[n][i]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n) p[n] = __builtin_bit_cast(bf16x8, q[n]);
+    }
+  }
+};
+
+// The adapters among a tile's rows, and the rank blocks of each, one after the other.
+struct Cursor {
+  uint32_t rest;  // rows whose adapter has not begun
+  uint32_t same;  // rows of the present one; 0 past the last
+  uint32_t slot, block, rank;
+  __device__ __forceinline__ void adapter(uint32_t ids, uint32_t ranks) {
+    const uint32_t at = rest ? (uint32_t)__builtin_ctz(rest) : 0u;
+    const uint32_t a = (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)at);
+    const uint32_t r = (uint32_t)__builtin_amdgcn_readlane((int)ranks, (int)at);
+    same = (uint32_t)__ballot(ids == a) & rest;
+    rest &= ~same;
+    block = 0;
+    if (same) {  // past the last the addresses stay where they were
+      slot = a;
+      rank = r;
+    }
+  }
+  __device__ __forceinline__ void next(uint32_t ids, uint32_t ranks) {
+    if (same && (block + 1u) * kBlock < rank) ++block;
+    else adapter(ids, ranks);
+  }
+};
+
+// One wavefront: 32 rows x 32 TT outputs (lane n: outputs TT n .. TT n + TT - 1). The rows are the first operand, the
+// outputs the second, so a register holds one row's 32 TT outputs side by side over 32 lanes. Each adapter's product
+// is computed for all 32 rows and taken for its own.
+// The weights of the next PF (adapter, rank block) pairs are on their way while one is worked on.
+template <int WT, int YT, int TT, int PF>
+__global__ __launch_bounds__(kThreads, 2) void expand_kernel(oxs_lora_table t, oxs_lora_batch b, uint32_t row_tiles,
+                                                             uint32_t col_tiles, uint32_t vec) {
+  const uint32_t lane = threadIdx.x & 63u, n = lane & 31u, g = lane >> 5;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t id = blockIdx.x * kWaves + wave;
+  const uint32_t col = id / row_tiles, row0 = (id - col * row_tiles) * kRows;
+  if (col >= col_tiles) return;
+  const uint32_t my_row = min(row0 + n, b.batch - 1u);
+  uint32_t ids = b.adapters[my_row];
+  if (row0 + n >= b.batch) ids = OXS_LORA_NONE;
+  const uint32_t ranks = rank_of(t, ids);
+  const uint32_t live = (uint32_t)__ballot(ranks != 0u);
+  if (live == 0u) return;
+  const uint32_t all_blocks = rank_blocks(t.max_rank);
+  constexpr uint32_t kPieces = kBlock * kGroup;  // elements of a group's rank block
+  constexpr uint32_t kPerGroup = kGroup / (32u * TT);
+  // outputs 32 TT col + TT n + tt: piece (q, n') of its group with 4 n' + q = output % 128
+  const uint32_t out0 = col * 32u * TT + TT * n;
+  const uint32_t in_group = (col % kPerGroup) * 32u * TT + TT * n;
+  const Element<WT>* wb = (const Element<WT>*)t.b + (size_t)(col / kPerGroup) * all_blocks * kPieces +
+                          (g * 4u + in_group % 4u) * 256u + (in_group / 4u) * 8u;
+  const uint16_t* vb = (const uint16_t*)b.workspace + (size_t)my_row * all_blocks * (kValueBytes / 2) + g * 8u;
+
+  Cursor ahead;
+  ahead.rest = live;
+  ahead.slot = ahead.rank = 0;
+  ahead.adapter(ids, ranks);
+  Eight<WT> w[PF][TT];
+  Eight<OXS_DTYPE_BF16> v[PF][kPlanes];
+  uint32_t same[PF];
+  const auto fetch = [&](int i) {
+    const Element<WT>* p = wb + (size_t)ahead.slot * b_elements(t) + (size_t)ahead.block * kPieces;
+    const bool in = g == 0u || ahead.block * kBlock + 8u < ahead.rank;  // this half holds a rank
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+      if (in) w[i][tt] = load_eight<WT>(p + tt * 256u);
+      else w[i][tt] = Eight<WT>{};
+    }
+#pragma unroll
+    for (int q = 0; q < (int)kPlanes; ++q)
+      v[i][q] = load_eight<OXS_DTYPE_BF16>(vb + ahead.block * (kValueBytes / 2) + q * kBlock);
+    same[i] = ahead.same;
+    ahead.next(ids, ranks);
+  };
+#pragma unroll
+  for (int i = 0; i < PF; ++i) fetch(i);
+
+  // y, where a row has an adapter
+  const uint32_t mine = live >> (4u * g);  // bit 8 (r / 4) + r % 4: register r's row
+  using YE = Element<YT>;
+  YE* y = (YE*)b.y + (size_t)row0 * (size_t)b.y_ld + out0;
+  const bool whole = vec && out0 + TT <= t.m;
+  YE old[16][TT];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    if (!((mine >> (8 * (r / 4) + r % 4)) & 1u)) continue;
+    const YE* p = y + (size_t)out_row(r, g) * (size_t)b.y_ld;
+    if (whole) {
+      struct alignas(TT * sizeof(YE)) Vec { YE e[TT]; };
+      const Vec q = *(const Vec*)p;
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) old[r][tt] = q.e[tt];
+    } else {
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) old[r][tt] = out0 + tt < t.m ? p[tt] : 0;
+    }
+  }
+
+  f32x16 acc[TT];
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) acc[tt] = (f32x16){};
+  do {
+#pragma unroll
+    for (int i = 0; i < PF; ++i) {
+      const uint32_t s = same[i];
+      if (s) {
+        bf16x8 vp[kPlanes];
+#pragma unroll
+        for (int q = 0; q < (int)kPlanes; ++q) vp[q] = __builtin_bit_cast(bf16x8, v[i][q].q[0]);
+        const uint32_t bits = s >> (4u * g);
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+          const Parts<WT> wp(w[i][tt]);
+          f32x16 d = s == live ? acc[tt] : (f32x16){};
+#pragma unroll
+          for (int sum = 2; sum >= 0; --sum)  // the small products first
+#pragma unroll
+            for (int q = 0; q < Parts<WT>::N; ++q)
+              if (q <= sum) d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vp[sum - q], wp.p[q], d, 0, 0, 0);
+          if (s == live) {
+            acc[tt] = d;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[tt][r] += (bits >> (8 * (r / 4) + r % 4)) & 1u ? d[r] : 0.0f;
+          }
+        }
+      }
+      fetch(i);
+    }
+  } while (same[0]);
+
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    if (!((mine >> (8 * (r / 4) + r % 4)) & 1u)) continue;
+    YE* p = y + (size_t)out_row(r, g) * (size_t)b.y_ld;
+    YE out[TT];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+      const float z = widen<YT>(old[r][tt]) + acc[tt][r];
+      if constexpr (YT == OXS_DTYPE_F32) out[tt] = __float_as_uint(z);
+      else out[tt] = (uint16_t)(narrow2(z, 0.0f) & 0xffffu);
+    }
+    if (whole) {
+      struct alignas(TT * sizeof(YE)) Vec { YE e[TT]; };
+      Vec q;
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) q.e[tt] = out[tt];
+      *(Vec*)p = q;
+    } else {
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt)
+        if (out0 + tt < t.m) p[tt] = out[tt];
+    }
+  }
 }
 
 static bool known(int32_t dt, bool half) {
@@ -113,9 +401,9 @@ static void by_values(int32_t dt, F f) {
 extern "C" int oxs_lora_table_bytes(const oxs_lora_table* table, size_t* a_bytes, size_t* b_bytes) {
   using namespace oxs_lora;
   if (!sizes_ok(table) || !a_bytes || !b_bytes) return OXS_ERR_INVALID_ARGUMENT;
-  const size_t per = (size_t)table->max_adapters * table->max_rank * size_of(table->dtype);
-  *a_bytes = per * table->k;
-  *b_bytes = per * table->m;
+  const size_t per = (size_t)table->max_adapters * size_of(table->dtype);
+  *a_bytes = per * a_elements(*table);
+  *b_bytes = per * b_elements(*table);
   return OXS_OK;
 }
 
@@ -129,8 +417,9 @@ extern "C" int oxs_lora_load(const oxs_lora_table* table, uint32_t slot, const v
     if ((rank > 1 && a_ld < (int64_t)table->k) || (table->m > 1 && b_ld < (int64_t)rank)) return OXS_ERR_INVALID_ARGUMENT;
   }
   by_weights(table->dtype, [&](auto wt) {
+    using E = Element<decltype(wt)::value>;
     hipLaunchKernelGGL(load_kernel<decltype(wt)::value>, dim3(1024), dim3(kThreads), 0, (hipStream_t)stream, *table,
-                       slot, a, a_ld, b, b_ld, rank, scale);
+                       slot, (const E*)a, a_ld, (const E*)b, b_ld, rank, scale);
   });
   return launched();
 }
@@ -138,7 +427,7 @@ extern "C" int oxs_lora_load(const oxs_lora_table* table, uint32_t slot, const v
 extern "C" size_t oxs_lora_workspace_bytes(const oxs_lora_table* table, uint32_t batch) {
   using namespace oxs_lora;
   if (!sizes_ok(table) || batch > 65536u) return 0;
-  return (size_t)(batch ? batch : 1u) * table->max_rank * 4u;
+  return (size_t)(batch ? batch : 1u) * rank_blocks(table->max_rank) * kValueBytes;
 }
 
 extern "C" int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* batch, void* stream) {
@@ -154,17 +443,26 @@ extern "C" int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* b
   if (!aligned(b.x, size_of(b.x_dtype)) || !aligned(b.y, size_of(b.y_dtype)) || !aligned(b.adapters, 4) ||
       !aligned(b.workspace, 16) || b.workspace_bytes < oxs_lora_workspace_bytes(table, b.batch))
     return OXS_ERR_INVALID_ARGUMENT;
-  const uint64_t grid = (uint64_t)((t.m + kThreads - 1) / kThreads) * b.batch;
-  if (grid >= (1u << 24)) return OXS_ERR_LIMITS;
+  if ((uint64_t)b.batch * t.m > (1ull << 31)) return OXS_ERR_LIMITS;
+  const hipStream_t st = (hipStream_t)stream;
+  const uint32_t row_tiles = (b.batch + kRows - 1u) / kRows;
+  const uint32_t ranks = rank_blocks(t.max_rank) * kBlock;
+  const auto even = [](const void* p, int64_t ld, uint32_t es, uint32_t to) {
+    return aligned(p, to) && ((uint64_t)ld * es) % to == 0;
+  };
   by_weights(t.dtype, [&](auto wt) {
     constexpr int WT = decltype(wt)::value;
     by_values(b.x_dtype, [&](auto xt) {
-      hipLaunchKernelGGL((shrink_kernel<WT, decltype(xt)::value>), dim3(b.batch, (t.max_rank + 3) / 4), dim3(kThreads),
-                         0, (hipStream_t)stream, t, b);
+      constexpr int XT = decltype(xt)::value;
+      const uint32_t vec = even(b.x, b.x_ld, size_of(XT), 16) ? 1u : 0u;
+      hipLaunchKernelGGL((shrink_kernel<WT, XT, 1>), dim3(b.batch, ranks / kWaves), dim3(kThreads), 0, st, t, b, vec);
     });
     by_values(b.y_dtype, [&](auto yt) {
-      hipLaunchKernelGGL((expand_kernel<WT, decltype(yt)::value>), dim3((uint32_t)grid), dim3(kThreads), 0,
-                         (hipStream_t)stream, t, b);
+      constexpr int YT = decltype(yt)::value, TT = 2;
+      const uint32_t col_tiles = (t.m + 32u * TT - 1u) / (32u * TT);
+      const uint32_t vec = even(b.y, b.y_ld, size_of(YT), TT * size_of(YT)) ? 1u : 0u;
+      hipLaunchKernelGGL((expand_kernel<WT, YT, TT, 4>), dim3((row_tiles * col_tiles + kWaves - 1u) / kWaves),
+                         dim3(kThreads), 0, st, t, b, row_tiles, col_tiles, vec);
     });
   });
   return launched();
