@@ -14,9 +14,15 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/oxide_sampler.h"
 
 namespace oxs_lp {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
@@ -214,107 +220,245 @@ __device__ __forceinline__ uint32_t keep_largest(uint64_t* keys, uint32_t count,
 
 // ---------------------------------------------------------------- the pass over the logits
 
-// G consecutive logits in one 16-byte load; a thread holds E of a tile as E / G groups that lie
-// kThreads * G apart. Rows that do not begin on 16 bytes are cut at the boundaries all the same: the
-// first and the last group of a row are then loaded one by one.
+// The parameters as they lie in memory, for what is needed after the pass only: read where they are used, they take
+// no scalar registers during it.
+__device__ __forceinline__ const Params& late_params() {
+  uint64_t q = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(q));
+  return *(const Params*)(const __attribute__((address_space(4))) Params*)q;
+}
+
+// A number of which the compiler knows nothing, so that what is computed from it in a rare branch is not kept in
+// registers all the time.
+__device__ __forceinline__ int32_t apart(int32_t x) {
+  asm("" : "+v"(x));
+  return x;
+}
+
+// The largest of N floats by their bits, as whole numbers: those of one sign are in the order of their magnitudes, so
+// it is the largest signed number if that has no sign bit, else the smallest unsigned one. One instruction per value
+// (half of one for pairs of bf16), where a maximum of floats takes one and a half, as it has to make signalling NaNs
+// quiet first. NaN if a positive NaN, or nothing but negative ones, is among them.
+template <int N>
+__device__ __forceinline__ float largest_of(const float* v) {
+  int32_t hi = (int32_t)__float_as_uint(v[0]);
+  uint32_t lo = __float_as_uint(v[0]);
+#pragma unroll
+  for (int e = 1; e < N; ++e) {
+    hi = max(hi, (int32_t)__float_as_uint(v[e]));
+    lo = min(lo, __float_as_uint(v[e]));
+  }
+  return __uint_as_float(hi >= 0 ? (uint32_t)hi : lo);
+}
+__device__ __forceinline__ float largest_of_pairs(u32x4 raw) {
+  const uint32_t first = raw[0];
+  i16x2 hi = __builtin_bit_cast(i16x2, first);
+  u16x2 lo = __builtin_bit_cast(u16x2, first);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    const uint32_t x = raw[i];  // (a bit cast of the element itself takes element 0)
+    hi = __builtin_elementwise_max(hi, __builtin_bit_cast(i16x2, x));
+    lo = __builtin_elementwise_min(lo, __builtin_bit_cast(u16x2, x));
+  }
+  const int32_t h = max((int32_t)hi[0], (int32_t)hi[1]);
+  return __uint_as_float((h >= 0 ? (uint32_t)h : (uint32_t)min(lo[0], lo[1])) << 16);
+}
+
+// A thread's sums s = sum 2^q, t = sum q 2^q with q = (y - ref) c for its logits' y. ref follows the largest logit
+// only when that is 2^kSlack away: the sums stay far from overflow, and most steps need no rescaling.
+// q is y c - (ref c rounded) in one operation. What that rounding leaves out (rest) is the same for all terms, so it
+// comes off the sums when ref changes.
+constexpr float kSlack = 16.0f;
+constexpr float kHuge = 1e31f;  // y c cannot overflow below this, as c <= 10^6 log2 e
+struct Sums {
+  float ref = -__builtin_inff(), rc = 0.0f, s = 0.0f, t = 0.0f;
+  __device__ __forceinline__ float rest(float c) const { return fabsf(ref) < kHuge ? __builtin_fmaf(ref, c, -rc) : 0.0f; }
+  __device__ __forceinline__ void shift(float by) {  // q + by in the place of q
+    const float f = exp2_fast(by);
+    t = f * __builtin_fmaf(by, s, t);
+    s = f * s;
+  }
+  // makes s and t relative to `to` >= ref itself, or (settled = false) to what the next terms are relative to
+  __device__ __forceinline__ void rebase(float to, float c, bool settled = false) {
+    shift(-rest(c));
+    shift(fmaxf((ref - to) * c, kFloor));  // (NaN, of two -inf: kFloor)
+    ref = to;
+    rc = ref * c;
+    if (settled) return;
+    shift(rest(c));
+  }
+  __device__ __forceinline__ bool behind(float top, float c) const {
+    return (top - ref) * c > kSlack || (ref == neg_inf() && top > ref);
+  }
+  __device__ __forceinline__ bool huge() const { return fabsf(ref) >= kHuge && ref > neg_inf(); }
+  // N more logits, of which none is 2^kSlack above ref
+  template <int N, class Y>
+  __device__ __forceinline__ void add(const float* v, float c, Y y) {
+    float s1 = 0.0f, t1 = 0.0f;
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const float q0 = fmaxf(__builtin_fmaf(y(v[e]), c, -rc), kFloor);
+      const float q1 = fmaxf(__builtin_fmaf(y(v[e + 1]), c, -rc), kFloor);
+      const float p0 = exp2_fast(q0), p1 = exp2_fast(q1);
+      s += p0;
+      s1 += p1;
+      t = __builtin_fmaf(q0, p0, t);
+      t1 = __builtin_fmaf(q1, p1, t1);
+    }
+    s += s1;
+    t += t1;
+  }
+};
+
+// G consecutive logits in one 16-byte load; a thread holds E of a tile as E / G groups that lie kThreads * G apart.
+// Rows that do not begin on 16 bytes are cut at the boundaries all the same, and the tile in which a row begins or
+// ends between two boundaries is loaded logit by logit.
 template <int DT>
 constexpr int group_size() { return DT == OXS_DTYPE_F32 ? 4 : 8; }
 
-template <int DT, int E, bool MASK, bool CAP>
-__global__ __launch_bounds__(kThreads) void rows_kernel(Params p) {
+template <int DT, int E, bool MASK, bool CAP, bool TOP>
+__global__ __launch_bounds__(kThreads, 5) void rows_kernel(Params p) {
   constexpr int G = group_size<DT>(), NG = E / G;
+  constexpr uint32_t kSize = DT == OXS_DTYPE_F32 ? 4 : 2;
   constexpr uint32_t kTile = kThreads * E;
+  constexpr int kStep = 8;  // logits that are summed while the next are still on their way
   const oxs_logprobs& b = p.b;
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t row = blockIdx.x / p.splits, part = blockIdx.x - row * p.splits;
-  const uint32_t V = b.vocab, T = b.tokens_per_row, N = b.top_n;
-  __shared__ uint64_t s_keys[kWaves][kRoom];
-  __shared__ uint32_t s_order[2][kThreads];
-  __shared__ uint64_t s_list[kThreads];
+  const uint32_t V = b.vocab, T = b.tokens_per_row, N = TOP ? b.top_n : 0u;
+  __shared__ uint64_t s_keys[TOP ? kWaves : 1][TOP ? kRoom : 1];
+  __shared__ uint32_t s_order[2][TOP ? kThreads : 1];
+  __shared__ uint64_t s_list[TOP ? kThreads : 1];
   __shared__ float s_m[kWaves], s_s[kWaves], s_t[kWaves];
   __shared__ uint32_t s_count[kWaves];
   __shared__ uint32_t s_before[kWaves][OXS_LOGPROBS_MAX_TOKENS];
 
-  const char* base = (const char*)b.logits + (size_t)row * (size_t)b.logits_ld * (DT == OXS_DTYPE_F32 ? 4 : 2);
+  const char* base = (const char*)b.logits + (size_t)row * (size_t)b.logits_ld * kSize;
   // logits between the boundary before the row and its first one
-  const uint32_t skip = ((uint32_t)(uintptr_t)base & 15u) / (DT == OXS_DTYPE_F32 ? 4 : 2);
+  const uint32_t skip = ((uint32_t)(uintptr_t)base & 15u) / kSize;
   const uint32_t* mask = MASK ? b.allowed_mask + (size_t)row * (size_t)b.mask_ld : nullptr;
   const float inv = inverse_temperature(b, row), c = inv * kLog2e;
   const float cap = b.logit_softcap, inv_cap = CAP ? 1.0f / cap : 0.0f;
+  const auto y_of = [&](float l) {
+    if constexpr (CAP) return l == neg_inf() ? l : softcap_of(l, cap, inv_cap);
+    else return l;
+  };
 
-  // lane j's given token
-  uint32_t want = kNoToken;
-  float want_l = neg_inf();
+  // lane j's given token; its logit (and mask word) are used after the first tile's
+  uint32_t want = kNoToken, want_bits = 0, want_word = 0;
   if (lane < T) want = b.tokens[(size_t)row * (size_t)b.tokens_ld + lane];
-
-  float m = neg_inf(), s = 0.0f, t = 0.0f;  // this thread's
-  float floor = neg_inf();                  // every alternative of the row is above it
-  float bound = neg_inf();                  // and those of this wavefront's tokens to come above this
-  uint32_t count = 0, round = 0;            // candidates of this wavefront; times the bound was raised
-  uint64_t* keys = s_keys[wave];
   if (lane < T) s_before[wave][lane] = 0;
+  float want_l = neg_inf();
+
+  Sums sums;
+  float m = neg_inf();      // the thread's largest logit
+  float floor = neg_inf();  // every alternative of the row is above it,
+  float bound = neg_inf();  // and those of this wavefront's tokens to come above this
+  uint32_t count = 0, round = 0;  // candidates of this wavefront; times the floor was raised
+  uint64_t* keys = s_keys[TOP ? wave : 0];
 
   const uint32_t first = part * p.tiles;
   const uint32_t total = (V + skip + kTile - 1u) / kTile;
   const uint32_t last = min(first + p.tiles, total);
   for (uint32_t tile = first; tile < last; ++tile) {
     // element e of group g is token at + g * kThreads * G + e (negative before the row: none)
-    const int64_t at0 = (int64_t)tile * kTile + tid * G - (int64_t)skip;
-    const int32_t at = (int32_t)at0;  // V <= 2^30
+    const int32_t at = (int32_t)(tile * kTile + tid * G - skip);  // V <= 2^30
+    const int64_t begin = (int64_t)tile * kTile - (int64_t)skip;  // of the tile
     float v[E];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const int32_t i = at + g * kThreads * G;
-      if (i >= 0 && i + G <= (int32_t)V) {
-        if constexpr (DT == OXS_DTYPE_F32) {
-          typedef float f4 __attribute__((ext_vector_type(4)));
-          const f4 x = __builtin_nontemporal_load((const f4*)(base + (int64_t)i * 4));
-#pragma unroll
-          for (int e = 0; e < G; ++e) v[g * G + e] = x[e];
-        } else {
-          typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-          const u4 x = __builtin_nontemporal_load((const u4*)(base + (int64_t)i * 2));
-#pragma unroll
-          for (int e = 0; e < G; ++e)
-            v[g * G + e] = __uint_as_float((e & 1) ? x[e >> 1] & 0xffff0000u : x[e >> 1] << 16);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < G; ++e) {
-          v[g * G + e] = neg_inf();
-          if (i + e >= 0 && i + e < (int32_t)V) {
-            if constexpr (DT == OXS_DTYPE_F32) v[g * G + e] = ((const float*)base)[i + e];
-            else v[g * G + e] = __uint_as_float((uint32_t)((const uint16_t*)base)[i + e] << 16);
-          }
-        }
-      }
-    }
-    if constexpr (MASK) {
+    const auto masked = [&](int g) {  // group g's logits that the mask leaves out become -inf
       const uint32_t words = (V + 31u) / 32u;
+      const int32_t i = max(at + g * kThreads * G, 0);  // (before the row: -inf already; its bits are those from 0 on)
+      const int32_t d = i - (at + g * kThreads * G);
+      const uint32_t w = min((uint32_t)i >> 5, words - 1u);
+      uint32_t bits = mask[w] >> (i & 31);
+      if ((i & 31) > 32 - G && w + 1u < words) bits |= mask[w + 1u] << (32 - (i & 31));
+      bits <<= d;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const int32_t i = max(at + g * kThreads * G, 0);  // (before the row: -inf already; its bits are those from 0 on)
-        const int32_t d = i - (at + g * kThreads * G);
-        const uint32_t w = min((uint32_t)i >> 5, words - 1u);
-        uint32_t bits = mask[w] >> (i & 31);
-        if ((i & 31) > 32 - G && w + 1u < words) bits |= mask[w + 1u] << (32 - (i & 31));
-        bits <<= d;
+      for (int e = 0; e < G; ++e)
+        if (!((bits >> e) & 1u)) v[g * G + e] = neg_inf();
+    };
+    u32x4 raw[NG];
+    if (begin >= 0 && begin + kTile <= (int64_t)V) {
 #pragma unroll
-        for (int e = 0; e < G; ++e)
-          if (!((bits >> e) & 1u)) v[g * G + e] = neg_inf();
+      for (int g = 0; g < NG; ++g)
+        raw[g] = __builtin_nontemporal_load((const u32x4*)(base + (uint32_t)(at + g * kThreads * G) * kSize));
+    } else {  // the row begins or ends in the tile: logit by logit, -inf outside
+      const int32_t mine = apart(at);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int32_t i = mine + (e / G) * kThreads * G + e % G;
+        const uint32_t j = (uint32_t)min(max(i, 0), (int32_t)V - 1);
+        if constexpr (DT == OXS_DTYPE_F32) {
+          const uint32_t x = *(const uint32_t*)(base + j * kSize);
+          raw[e / G][e % G] = i == (int32_t)j ? x : 0xff800000u;
+        } else {
+          uint32_t x = *(const uint16_t*)(base + j * kSize);
+          x = i == (int32_t)j ? x : 0xff80u;
+          if (e & 1) raw[e / G][(e % G) >> 1] |= x << 16;
+          else raw[e / G][(e % G) >> 1] = x;
+        }
+        if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // (the addresses of all at once would not fit)
       }
     }
-    if (tile == first && lane < T) want_l = present_logit<DT>(b, row, want);
-
-    // the thread's largest (the maximum passes over quiet NaNs only)
-    float top = __builtin_canonicalizef(v[0]);
+    if (tile == first && want < V) {
+      if constexpr (DT == OXS_DTYPE_F32) want_bits = *(const uint32_t*)(base + want * kSize);
+      else want_bits = (uint32_t)*(const uint16_t*)(base + want * kSize) << 16;
+      if constexpr (MASK) want_word = mask[want >> 5];
+    }
+    const Sums before_tile = sums;
+    float top = neg_inf();  // the thread's largest of the tile
+    float tops[E / kStep];
+    bool odd = false;
 #pragma unroll
-    for (int e = 1; e < E; ++e) top = fmaxf(top, v[e]);
-    const float old = m;
+    for (int e0 = 0; e0 < E; e0 += kStep) {
+#pragma unroll
+      for (int e = e0; e < e0 + kStep; ++e) {
+        if constexpr (DT == OXS_DTYPE_F32) v[e] = __uint_as_float(raw[e / G][e % G]);
+        else v[e] = __uint_as_float((e & 1) ? raw[e / G][(e % G) >> 1] & 0xffff0000u : raw[e / G][(e % G) >> 1] << 16);
+      }
+      float x;
+      if constexpr (MASK) {
+#pragma unroll
+        for (int g = e0 / G; g < (e0 + kStep) / G; ++g) masked(g);
+      }
+      if constexpr (DT == OXS_DTYPE_BF16 && !MASK) x = largest_of_pairs(raw[e0 / G]);
+      else x = largest_of<kStep>(v + e0);
+      odd |= x != x;
+      tops[e0 / kStep] = x;
+      top = fmaxf(top, x);
+      const float y = y_of(x);
+      if (__ballot(sums.behind(y, c))) sums.rebase(fmaxf(sums.ref, y), c);
+      sums.add<kStep>(v + e0, c, y_of);
+      __builtin_amdgcn_sched_barrier(0);  // nothing waits for the loads of later steps
+    }
+    const bool slow = __ballot(odd || sums.huge()) != 0;
+    if (__builtin_expect(slow, 0)) {
+      // NaNs among the logits may have hidden the largest, and a huge one (a mask of the type's lowest value, say)
+      // makes y c overflow: the tile again, from memory, logit by logit and with the difference first.
+      sums = before_tile;
+      top = neg_inf();
+#pragma unroll 1
+      for (int e = 0; e < E; ++e)
+        top = fmaxf(top, present_logit<DT>(b, row, (uint32_t)(at + (e / G) * kThreads * G + e % G)));
+      sums.rebase(fmaxf(sums.ref, y_of(top)), c, true);
+#pragma unroll 1
+      for (int e = 0; e < E; ++e) {
+        const float y = y_of(present_logit<DT>(b, row, (uint32_t)(at + (e / G) * kThreads * G + e % G)));
+        const float q = fmaxf((y - sums.ref) * c, kFloor), f = exp2_fast(q);
+        sums.s += f;
+        sums.t = __builtin_fmaf(q, f, sums.t);
+      }
+      sums.shift(sums.rest(c));
+    }
     m = fmaxf(m, top);
+    if (tile == first && want < V) {
+      const float l = __uint_as_float(want_bits);
+      const bool in = !MASK || ((want_word >> (want & 31u)) & 1u);
+      want_l = l == l && in ? l : neg_inf();
+    }
 
-    if (N) {
+    if constexpr (TOP) {
       // Raise the floor at the 1st, 2nd, 4th, ... and last tile: at least N logits so far are no less than
       // the N-th largest of the 256 threads' maxima, so the rest cannot be alternatives.
       const uint32_t n = tile - first + 1u;
@@ -326,8 +470,16 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(Params p) {
         uint32_t o[kWaves];
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) o[w] = so[w * 64 + lane];
-        uint32_t lo = kOrderNegInf, hi = 0xffffffffu;  // N maxima are >= lo, fewer are >= hi
-        for (int step = 0; step < 32 && hi - lo > 1u; ++step) {
+        uint32_t lo = o[0], hi = o[0];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) {
+          lo = min(lo, o[w]);
+          hi = max(hi, o[w]);
+        }
+        lo = wave_reduce(lo, 0xffffffffu, [](uint32_t x, uint32_t y) { return min(x, y); });
+        hi = wave_reduce(hi, 0u, [](uint32_t x, uint32_t y) { return max(x, y); }) + 1u;
+        // at least N maxima are >= lo, fewer are >= hi
+        for (int i = 0; i < 32 && hi - lo > 1u; ++i) {
           const uint32_t mid = lo + (hi - lo) / 2u;
           uint32_t k = 0;
 #pragma unroll
@@ -339,55 +491,41 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(Params p) {
         floor = fmaxf(floor, just_below(lo));
         bound = fmaxf(bound, floor);
       }
-      if (__ballot(top > bound)) {
+      const auto push = [&](float x, uint32_t id) {
+        const uint64_t who = __ballot(x > bound);
+        if (!who) return;
+        if (x > bound)
+          keys[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u))] =
+              key_of(x, id);
+        count += (uint32_t)__popcll(who);
+      };
+      const uint32_t lanes = (uint32_t)__popcll(__ballot(top > bound));
+      if (lanes != 0u && count + lanes * E <= kRoom && !slow) {
+        const uint32_t mine = (uint32_t)apart(at);
 #pragma unroll
+        for (int e0 = 0; e0 < E; e0 += kStep) {
+          if (!__ballot(tops[e0 / kStep] > bound)) continue;
+#pragma unroll
+          for (int e = e0; e < e0 + kStep; ++e) push(v[e], mine + (uint32_t)((e / G) * kThreads * G + e % G));
+        }
+      } else if (lanes != 0u) {
+        // More candidates than room, perhaps (many equal logits, a row that rises, few tokens allowed): group by
+        // group from memory, keeping the N largest whenever the next group might not fit.
+#pragma unroll 1
         for (int g = 0; g < NG; ++g) {
-          float gm = v[g * G];
-#pragma unroll
-          for (int e = 1; e < G; ++e) gm = fmaxf(gm, v[g * G + e]);
-          if (!__ballot(gm > bound)) continue;
-          if (count + 64u * G > kRoom) {  // room for the whole group
+          if (count + 64u * G > kRoom) {
             count = keep_largest(keys, count, N);
             // later tokens of this wavefront have larger ids: equal ones come after
             if (count == N) bound = fmaxf(bound, key_value(keys[N - 1u]));
           }
+          const uint32_t i = (uint32_t)(at + g * kThreads * G);
+          float x[G];
 #pragma unroll
-          for (int e = 0; e < G; ++e) {
-            const float x = v[g * G + e];
-            const uint64_t who = __ballot(x > bound);
-            if (who) {
-              if (x > bound)
-                keys[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32),
-                                                       __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u))] =
-                    key_of(x, (uint32_t)(at + g * kThreads * G + e));
-              count += (uint32_t)__popcll(who);
-            }
-          }
+          for (int e = 0; e < G; ++e) x[e] = present_logit<DT>(b, row, i + e);
+#pragma unroll
+          for (int e = 0; e < G; ++e) push(x[e], i + e);
         }
       }
-    }
-
-    {  // s and t, relative to the thread's new maximum
-      const float y_m = capped<CAP>(m, cap, inv_cap);
-      const float d = fmaxf((capped<CAP>(old, cap, inv_cap) - y_m) * c, kFloor), f = exp2_fast(d);
-      float s0 = f * s, t0 = f * __builtin_fmaf(d, s, t), s1 = 0.0f, t1 = 0.0f;
-      if (old == neg_inf()) s0 = t0 = 0.0f;
-#pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float q0 = fmaxf((capped<CAP>(v[e], cap, inv_cap) - y_m) * c, kFloor);
-        const float q1 = fmaxf((capped<CAP>(v[e + 1], cap, inv_cap) - y_m) * c, kFloor);
-        float p0 = exp2_fast(q0), p1 = exp2_fast(q1);
-        if constexpr (CAP) {  // the cap of -inf is a value
-          p0 = v[e] == neg_inf() ? 0.0f : p0;
-          p1 = v[e + 1] == neg_inf() ? 0.0f : p1;
-        }
-        s0 += p0;
-        s1 += p1;
-        t0 = __builtin_fmaf(q0, p0, t0);
-        t1 = __builtin_fmaf(q1, p1, t1);
-      }
-      s = s0 + s1;
-      t = t0 + t1;
     }
 
     // tokens in front of the given ones
@@ -395,42 +533,35 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(Params p) {
       const float l = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(want_l), (int)j));
       if (l == neg_inf()) continue;
       const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)want, (int)j);
-      const uint64_t begin = (uint64_t)tile * kTile;  // of the tile, in tokens + skip
+      const float below = just_below(order_of(l));  // a logit of an earlier token counts from l on, of a later one above
       uint32_t k = 0;
-      if (begin + kTile <= (uint64_t)id + skip) {
+      if (begin + kTile <= (int64_t)id || begin > (int64_t)id) {
+        const float than = begin > (int64_t)id ? l : below;
 #pragma unroll
-        for (int e = 0; e < E; ++e) k += v[e] >= l ? 1u : 0u;
-      } else if (begin > (uint64_t)id + skip) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) k += v[e] > l ? 1u : 0u;
+        for (int e = 0; e < E; ++e) k += (uint32_t)__popcll(__ballot(v[e] > than));
       } else {
+        const int32_t to = (int32_t)id - apart(at);  // element e is before the token if its offset is below
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
-#pragma unroll
-          for (int e = 0; e < G; ++e) {
-            const bool lower = at + g * kThreads * G + e < (int32_t)id;
-            const float x = v[g * G + e];
-            k += (x > l || (x == l && lower)) ? 1u : 0u;
-          }
+        for (int e = 0; e < E; ++e)
+          k += (uint32_t)__popcll(__ballot(v[e] > ((e / G) * kThreads * G + e % G < to ? below : l)));
       }
-      k = wave_sum(k);
       if (lane == j) s_before[wave][j] += k;
     }
   }
 
-  // the workgroup's sums
+  // the workgroup's sums, relative to its largest logit
+  const Params& late = late_params();
+  const float wm = wave_max(m);
+  sums.rebase(fmaxf(y_of(wm), sums.ref), c, true);
   {
-    const float wm = wave_max(m), y_m = capped<CAP>(wm, cap, inv_cap);
-    const float d = fmaxf((capped<CAP>(m, cap, inv_cap) - y_m) * c, kFloor);
-    const float f = m == neg_inf() ? 0.0f : exp2_fast(d);
-    const float ws = wave_sum(f * s), wt = wave_sum(f * __builtin_fmaf(d, s, t));
+    const float ws = wave_sum(sums.s), wt = wave_sum(sums.t);
     if (lane == 0) {
       s_m[wave] = wm;
       s_s[wave] = ws;
       s_t[wave] = wt;
     }
   }
-  if (N) {
+  if constexpr (TOP) {
     // drop what the last floor leaves out, and keep at most 64 candidates per wavefront
     uint32_t kept = 0;
     for (uint32_t i0 = 0; i0 < count; i0 += 64u) {
@@ -449,20 +580,17 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(Params p) {
   __syncthreads();
   float bm = s_m[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) bm = s_m[w] > bm ? s_m[w] : bm;
+  for (int w = 1; w < kWaves; ++w) bm = fmaxf(bm, s_m[w]);
   float bs = 0.0f, bt = 0.0f;
-  {
-    const float y_m = capped<CAP>(bm, cap, inv_cap);
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float d = fmaxf((capped<CAP>(s_m[w], cap, inv_cap) - y_m) * c, kFloor);
-      const float f = s_m[w] == neg_inf() ? 0.0f : exp2_fast(d);
-      bs += f * s_s[w];
-      bt += f * __builtin_fmaf(d, s_s[w], s_t[w]);
-    }
+  for (int w = 0; w < kWaves; ++w) {
+    const float d = fmaxf((y_of(s_m[w]) - y_of(bm)) * c, kFloor), f = exp2_fast(d);
+    bs += f * s_s[w];
+    bt += f * __builtin_fmaf(d, s_s[w], s_t[w]);
   }
-  uint32_t before_me = 0, all = 0;
-  if (N) {  // one list of the workgroup's candidates
+  uint32_t all = 0;
+  if constexpr (TOP) {  // one list of the workgroup's candidates
+    uint32_t before_me = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       if (w < (int)wave) before_me += s_count[w];
@@ -471,30 +599,31 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(Params p) {
     if (lane < count) s_list[before_me + lane] = keys[lane];
     __syncthreads();
   }
-  uint32_t before = 0;  // of given token tid
-  if (tid < T)
+  uint32_t before = 0;  // tokens of this part in front of given token tid
+  if (tid < T) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) before += s_before[w][tid];
+  }
   uint64_t mine = 0;
   uint32_t place = kNoToken;
-  if (tid < all) {
+  if (TOP && tid < all) {
     mine = s_list[tid];
     place = 0;
     for (uint32_t i = 0; i < all; ++i) place += s_list[i] > mine ? 1u : 0u;
   }
-  if (p.splits > 1u) {
-    const size_t at = (size_t)row * p.splits + part;
-    if (tid == 0) p.stats[at] = make_float4(bm, bs, bt, 0.0f);
-    if (tid < T) p.counts[at * T + tid] = before;
-    if (place < N) p.keys[at * N + place] = mine;
-    if (tid >= all && tid < N) p.keys[at * N + tid] = 0;
+  if (late.splits > 1u) {
+    const size_t at = (size_t)row * late.splits + part;
+    if (tid == 0) late.stats[at] = make_float4(bm, bs, bt, 0.0f);
+    if (tid < T) late.counts[at * T + tid] = before;
+    if (TOP && place < N) late.keys[at * N + place] = mine;
+    if (TOP && tid >= all && tid < N) late.keys[at * N + tid] = 0;
     return;
   }
-  const Row r(b, inv, bm, bs, bt);
-  if (tid == 0) r.write(b, row);
-  if (tid < T) r.write_token(b, row, tid, want_l, before);  // (T <= 64: the first wavefront)
-  if (place < N) r.write_top(b, row, place, mine);
-  if (tid >= all && tid < N) r.write_top(b, row, tid, 0);
+  const Row r(late.b, inv, bm, bs, bt);
+  if (tid == 0) r.write(late.b, row);
+  if (tid < T) r.write_token(late.b, row, tid, want_l, before);  // (T <= 64: the first wavefront)
+  if (TOP && place < N) r.write_top(late.b, row, place, mine);
+  if (TOP && tid >= all && tid < N) r.write_top(late.b, row, tid, 0);
 }
 
 // One wavefront joins the parts of a row. The alternatives are the keys no less than a bound that is
@@ -588,13 +717,18 @@ static void launch(Params& p, hipStream_t st) {
   p.splits = (tiles + p.tiles - 1u) / p.tiles;
   const dim3 grid(b.rows * p.splits);
   const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, p); };
-  if (b.allowed_mask) {
-    if (small) go(rows_kernel<DT, 8, true, CAP>);
-    else go(rows_kernel<DT, 32, true, CAP>);
-  } else {
-    if (small) go(rows_kernel<DT, 8, false, CAP>);
-    else go(rows_kernel<DT, 32, false, CAP>);
-  }
+  const auto by_top = [&](auto e, auto mask) {
+    constexpr int kE = decltype(e)::value;
+    constexpr bool kMask = decltype(mask)::value;
+    if (b.top_n) go(rows_kernel<DT, kE, kMask, CAP, true>);
+    else go(rows_kernel<DT, kE, kMask, CAP, false>);
+  };
+  const auto by_mask = [&](auto e) {
+    if (b.allowed_mask) by_top(e, std::true_type{});
+    else by_top(e, std::false_type{});
+  };
+  if (small) by_mask(std::integral_constant<int, 8>{});
+  else by_mask(std::integral_constant<int, 32>{});
   if (p.splits == 1u) return;
   const auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(b.rows), dim3(64), 0, st, p); };
   if (p.splits * b.top_n <= 5u * 64u) join(merge_kernel<DT, CAP, 5>);
