@@ -7,9 +7,8 @@
 // H's two terms are both >= 0, so nothing cancels. Differences to m are taken
 // before the scaling, so large logits lose nothing either.
 //
-// rows_kernel: a workgroup reads a part of a row in tiles that stay in
-// registers; each thread keeps its own m, s and t. merge_kernel: a wavefront
-// joins the parts of a row where it was split over workgroups (few rows).
+// rows_kernel: a workgroup reads a part of a row in tiles that stay in registers; each thread keeps its own m, s and
+// t. merge_kernel: a wavefront joins the parts of a row where it was split over workgroups (few rows).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -18,6 +17,18 @@
 
 #include "../../include/oxide_sampler.h"
 
+#ifndef LP_E
+#define LP_E 16
+#endif
+#ifndef LP_TARGET
+#define LP_TARGET 1024u
+#endif
+#ifndef LP_ROWS
+#define LP_ROWS 512u
+#endif
+#ifndef LP_OCC
+#define LP_OCC 5
+#endif
 namespace oxs_lp {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -31,7 +42,10 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.693147180559945309417f;
 // 2^-256 is 0 in 32 bits: a difference below this (or NaN, of two infinities) adds nothing
 constexpr float kFloor = -256.0f;
-constexpr uint32_t kMaxSplits = 64;      // parts of a row
+#ifndef LP_SPLITS
+#define LP_SPLITS 64
+#endif
+constexpr uint32_t kMaxSplits = LP_SPLITS;      // parts of a row
 constexpr uint32_t kMaxParts = 4096;     // rows * parts of a call that splits its rows
 constexpr uint32_t kMergeKeys = 20 * 64; // parts * top_n of a split row
 constexpr uint32_t kRoom = OXS_LOGPROBS_MAX_TOP + 512;  // candidates of a wavefront: those kept, and 64 lanes' next 8
@@ -96,6 +110,11 @@ __device__ __forceinline__ float wave_max(float x) {
   return __uint_as_float(wave_reduce(__float_as_uint(x), __float_as_uint(neg_inf()), [](uint32_t a, uint32_t b) {
     return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
   }));
+}
+
+// Lanes of `who` below this one.
+__device__ __forceinline__ uint32_t mbcnt(uint64_t who) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
 }
 
 // Orders a wavefront's accesses to LDS across its lanes.
@@ -317,7 +336,7 @@ template <int DT>
 constexpr int group_size() { return DT == OXS_DTYPE_F32 ? 4 : 8; }
 
 template <int DT, int E, bool MASK, bool CAP, bool TOP>
-__global__ __launch_bounds__(kThreads, 5) void rows_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
   constexpr int G = group_size<DT>(), NG = E / G;
   constexpr uint32_t kSize = DT == OXS_DTYPE_F32 ? 4 : 2;
   constexpr uint32_t kTile = kThreads * E;
@@ -327,7 +346,10 @@ __global__ __launch_bounds__(kThreads, 5) void rows_kernel(Params p) {
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t row = blockIdx.x / p.splits, part = blockIdx.x - row * p.splits;
   const uint32_t V = b.vocab, T = b.tokens_per_row, N = TOP ? b.top_n : 0u;
+  constexpr uint32_t kStage = 512 / E;  // threads whose logits are looked at together
   __shared__ uint64_t s_keys[TOP ? kWaves : 1][TOP ? kRoom : 1];
+  __shared__ __align__(16) float s_stage[TOP ? kWaves : 1][TOP ? 512 : 4];
+  __shared__ uint32_t s_stage_id[TOP ? kWaves : 1][TOP ? kStage : 1];
   __shared__ uint32_t s_order[2][TOP ? kThreads : 1];
   __shared__ uint64_t s_list[TOP ? kThreads : 1];
   __shared__ float s_m[kWaves], s_s[kWaves], s_t[kWaves];
@@ -348,8 +370,9 @@ __global__ __launch_bounds__(kThreads, 5) void rows_kernel(Params p) {
   // lane j's given token; its logit (and mask word) are used after the first tile's
   uint32_t want = kNoToken, want_bits = 0, want_word = 0;
   if (lane < T) want = b.tokens[(size_t)row * (size_t)b.tokens_ld + lane];
-  if (lane < T) s_before[wave][lane] = 0;
-  float want_l = neg_inf();
+  // a logit of an earlier token is in front from want_l on, of a later one above it
+  float want_l = neg_inf(), want_below = neg_inf();
+  uint32_t before = 0;  // tokens of this wavefront in front of lane j's
 
   Sums sums;
   float m = neg_inf();      // the thread's largest logit
@@ -357,10 +380,53 @@ __global__ __launch_bounds__(kThreads, 5) void rows_kernel(Params p) {
   float bound = neg_inf();  // and those of this wavefront's tokens to come above this
   uint32_t count = 0, round = 0;  // candidates of this wavefront; times the floor was raised
   uint64_t* keys = s_keys[TOP ? wave : 0];
+  float* stage = s_stage[TOP ? wave : 0];
+  uint32_t* stage_id = s_stage_id[TOP ? wave : 0];
 
   const uint32_t first = part * p.tiles;
   const uint32_t total = (V + skip + kTile - 1u) / kTile;
   const uint32_t last = min(first + p.tiles, total);
+  // a tile's logits, as they lie in memory; -inf outside the row
+  const auto fetch = [&](uint32_t tile, u32x4 (&to)[NG]) {
+    const int32_t at = (int32_t)(tile * kTile + tid * G - skip);
+    const int64_t begin = (int64_t)tile * kTile - (int64_t)skip;
+    if (begin >= 0 && begin + kTile <= (int64_t)V) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+        to[g] = __builtin_nontemporal_load((const u32x4*)(base + (uint32_t)(at + g * kThreads * G) * kSize));
+    } else {  // the row begins or ends in the tile: logit by logit
+      const int32_t mine = apart(at);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int32_t i = mine + (e / G) * kThreads * G + e % G;
+        const uint32_t j = (uint32_t)min(max(i, 0), (int32_t)V - 1);
+        if constexpr (DT == OXS_DTYPE_F32) {
+          const uint32_t x = *(const uint32_t*)(base + j * kSize);
+          to[e / G][e % G] = i == (int32_t)j ? x : 0xff800000u;
+        } else {
+          uint32_t x = *(const uint16_t*)(base + j * kSize);
+          x = i == (int32_t)j ? x : 0xff80u;
+          if (e & 1) to[e / G][(e % G) >> 1] |= x << 16;
+          else to[e / G][(e % G) >> 1] = x;
+        }
+        if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // (the addresses of all at once would not fit)
+      }
+    }
+  };
+  u32x4 raw[NG];
+  fetch(first, raw);
+  if (want < V) {
+    if constexpr (DT == OXS_DTYPE_F32) want_bits = *(const uint32_t*)(base + want * kSize);
+    else want_bits = (uint32_t)*(const uint16_t*)(base + want * kSize) << 16;
+    if constexpr (MASK) want_word = mask[want >> 5];
+  }
+  const auto want_set = [&]() {
+    const float l = __uint_as_float(want_bits);
+    const bool in = want < V && l == l && (!MASK || ((want_word >> (want & 31u)) & 1u));
+    want_l = in ? l : neg_inf();
+    want_below = just_below(order_of(want_l));
+  };
+  if (last <= first) want_set();  // a part past the row's end
   for (uint32_t tile = first; tile < last; ++tile) {
     // element e of group g is token at + g * kThreads * G + e (negative before the row: none)
     const int32_t at = (int32_t)(tile * kTile + tid * G - skip);  // V <= 2^30
@@ -378,37 +444,12 @@ __global__ __launch_bounds__(kThreads, 5) void rows_kernel(Params p) {
       for (int e = 0; e < G; ++e)
         if (!((bits >> e) & 1u)) v[g * G + e] = neg_inf();
     };
-    u32x4 raw[NG];
-    if (begin >= 0 && begin + kTile <= (int64_t)V) {
+    u32x4 next[NG];
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
-        raw[g] = __builtin_nontemporal_load((const u32x4*)(base + (uint32_t)(at + g * kThreads * G) * kSize));
-    } else {  // the row begins or ends in the tile: logit by logit, -inf outside
-      const int32_t mine = apart(at);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int32_t i = mine + (e / G) * kThreads * G + e % G;
-        const uint32_t j = (uint32_t)min(max(i, 0), (int32_t)V - 1);
-        if constexpr (DT == OXS_DTYPE_F32) {
-          const uint32_t x = *(const uint32_t*)(base + j * kSize);
-          raw[e / G][e % G] = i == (int32_t)j ? x : 0xff800000u;
-        } else {
-          uint32_t x = *(const uint16_t*)(base + j * kSize);
-          x = i == (int32_t)j ? x : 0xff80u;
-          if (e & 1) raw[e / G][(e % G) >> 1] |= x << 16;
-          else raw[e / G][(e % G) >> 1] = x;
-        }
-        if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // (the addresses of all at once would not fit)
-      }
-    }
-    if (tile == first && want < V) {
-      if constexpr (DT == OXS_DTYPE_F32) want_bits = *(const uint32_t*)(base + want * kSize);
-      else want_bits = (uint32_t)*(const uint16_t*)(base + want * kSize) << 16;
-      if constexpr (MASK) want_word = mask[want >> 5];
-    }
+    for (int g = 0; g < NG; ++g) next[g] = raw[g];
+    if (tile + 1u < last) fetch(tile + 1u, next);
     const Sums before_tile = sums;
     float top = neg_inf();  // the thread's largest of the tile
-    float tops[E / kStep];
     bool odd = false;
 #pragma unroll
     for (int e0 = 0; e0 < E; e0 += kStep) {
@@ -425,7 +466,6 @@ __global__ __launch_bounds__(kThreads, 5) void rows_kernel(Params p) {
       if constexpr (DT == OXS_DTYPE_BF16 && !MASK) x = largest_of_pairs(raw[e0 / G]);
       else x = largest_of<kStep>(v + e0);
       odd |= x != x;
-      tops[e0 / kStep] = x;
       top = fmaxf(top, x);
       const float y = y_of(x);
       if (__ballot(sums.behind(y, c))) sums.rebase(fmaxf(sums.ref, y), c);
@@ -452,17 +492,13 @@ __global__ __launch_bounds__(kThreads, 5) void rows_kernel(Params p) {
       sums.shift(sums.rest(c));
     }
     m = fmaxf(m, top);
-    if (tile == first && want < V) {
-      const float l = __uint_as_float(want_bits);
-      const bool in = !MASK || ((want_word >> (want & 31u)) & 1u);
-      want_l = l == l && in ? l : neg_inf();
-    }
+    if (tile == first) want_set();
 
     if constexpr (TOP) {
-      // Raise the floor at the 1st, 2nd, 4th, ... and last tile: at least N logits so far are no less than
+      // Raise the floor at the 1st, 4th, 16th, ... and last tile: at least N logits so far are no less than
       // the N-th largest of the 256 threads' maxima, so the rest cannot be alternatives.
       const uint32_t n = tile - first + 1u;
-      if ((n & (n - 1u)) == 0u || tile + 1u == last) {
+      if (((n & (n - 1u)) == 0u && (n & 0x55555555u)) || tile + 1u == last) {
         uint32_t* so = s_order[round & 1u];  // (a wavefront is at most one round ahead)
         ++round;
         so[tid] = order_of(m);
@@ -491,49 +527,51 @@ __global__ __launch_bounds__(kThreads, 5) void rows_kernel(Params p) {
         floor = fmaxf(floor, just_below(lo));
         bound = fmaxf(bound, floor);
       }
-      const auto push = [&](float x, uint32_t id) {
-        const uint64_t who = __ballot(x > bound);
-        if (!who) return;
-        if (x > bound)
-          keys[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u))] =
-              key_of(x, id);
-        count += (uint32_t)__popcll(who);
-      };
-      const uint32_t lanes = (uint32_t)__popcll(__ballot(top > bound));
-      if (lanes != 0u && count + lanes * E <= kRoom && !slow) {
-        const uint32_t mine = (uint32_t)apart(at);
-#pragma unroll
-        for (int e0 = 0; e0 < E; e0 += kStep) {
-          if (!__ballot(tops[e0 / kStep] > bound)) continue;
-#pragma unroll
-          for (int e = e0; e < e0 + kStep; ++e) push(v[e], mine + (uint32_t)((e / G) * kThreads * G + e % G));
-        }
-      } else if (lanes != 0u) {
-        // More candidates than room, perhaps (many equal logits, a row that rises, few tokens allowed): group by
-        // group from memory, keeping the N largest whenever the next group might not fit.
-#pragma unroll 1
-        for (int g = 0; g < NG; ++g) {
-          if (count + 64u * G > kRoom) {
-            count = keep_largest(keys, count, N);
-            // later tokens of this wavefront have larger ids: equal ones come after
-            if (count == N) bound = fmaxf(bound, key_value(keys[N - 1u]));
+      // The logits of the threads that have one above the bound go through LDS, kStage threads at a time, and every
+      // lane then looks at a few of them.
+      uint64_t rest = __ballot(top > bound);
+      float above = bound;
+      while (rest) {
+        if (count + min((uint32_t)__popcll(rest), kStage) * E > kRoom) {
+          count = keep_largest(keys, count, N);
+          if (count == N) {  // a lower id may still come in this tile, of the same logit
+            const float nth = key_value(keys[N - 1u]);
+            above = fmaxf(above, just_below(order_of(nth)));
+            bound = fmaxf(bound, nth);
           }
-          const uint32_t i = (uint32_t)(at + g * kThreads * G);
-          float x[G];
-#pragma unroll
-          for (int e = 0; e < G; ++e) x[e] = present_logit<DT>(b, row, i + e);
-#pragma unroll
-          for (int e = 0; e < G; ++e) push(x[e], i + e);
         }
+        const uint32_t to = mbcnt(rest);
+        const bool mine = ((rest >> lane) & 1u) && to < kStage;
+        if (mine) {
+#pragma unroll
+          for (int e = 0; e < E; e += 4)
+            *(float4*)&stage[to * E + e] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          stage_id[to] = (uint32_t)at;
+        }
+        const uint64_t sent = __ballot(mine);
+        rest &= ~sent;
+        const uint32_t n = (uint32_t)__popcll(sent) * E;
+        wave_sync();
+        for (uint32_t i0 = 0; i0 < n; i0 += 64u) {
+          const uint32_t i = i0 + lane, e = i % E;
+          const float x = i < n ? stage[i] : neg_inf();
+          const uint64_t who = __ballot(x > above);
+          if (!who) continue;
+          if (x > above)
+            keys[count + mbcnt(who)] = key_of(x, stage_id[i / E] + (e / G) * (kThreads * G) + e % G);
+          count += (uint32_t)__popcll(who);
+        }
+        wave_sync();
       }
     }
 
-    // tokens in front of the given ones
+    // Tokens in front of the given ones. (Counted through the scalar unit: a compare per logit on the vector unit,
+    // where adding up the lanes' counts would take another, and a sum over the lanes per tile.)
     for (uint32_t j = 0; j < T; ++j) {
       const float l = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(want_l), (int)j));
       if (l == neg_inf()) continue;
+      const float below = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(want_below), (int)j));
       const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)want, (int)j);
-      const float below = just_below(order_of(l));  // a logit of an earlier token counts from l on, of a later one above
       uint32_t k = 0;
       if (begin + kTile <= (int64_t)id || begin > (int64_t)id) {
         const float than = begin > (int64_t)id ? l : below;
@@ -545,13 +583,16 @@ __global__ __launch_bounds__(kThreads, 5) void rows_kernel(Params p) {
         for (int e = 0; e < E; ++e)
           k += (uint32_t)__popcll(__ballot(v[e] > ((e / G) * kThreads * G + e % G < to ? below : l)));
       }
-      if (lane == j) s_before[wave][j] += k;
+      if (lane == j) before += k;
     }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) raw[g] = next[g];
   }
 
   // the workgroup's sums, relative to its largest logit
   const Params& late = late_params();
   const float wm = wave_max(m);
+  if (lane < T) s_before[wave][lane] = before;
   sums.rebase(fmaxf(y_of(wm), sums.ref), c, true);
   {
     const float ws = wave_sum(sums.s), wt = wave_sum(sums.t);
@@ -562,19 +603,21 @@ __global__ __launch_bounds__(kThreads, 5) void rows_kernel(Params p) {
     }
   }
   if constexpr (TOP) {
-    // drop what the last floor leaves out, and keep at most 64 candidates per wavefront
-    uint32_t kept = 0;
-    for (uint32_t i0 = 0; i0 < count; i0 += 64u) {
-      const uint64_t k = i0 + lane < count ? keys[i0 + lane] : 0;
-      const bool in = k && key_value(k) > floor;
-      const uint64_t who = __ballot(in);
+    // drop what the last floor leaves out (all are above the only one), and keep at most 64 candidates per wavefront
+    if (round > 1u) {
+      uint32_t kept = 0;
+      for (uint32_t i0 = 0; i0 < count; i0 += 64u) {
+        const uint64_t k = i0 + lane < count ? keys[i0 + lane] : 0;
+        const bool in = k && key_value(k) > floor;
+        const uint64_t who = __ballot(in);
+        wave_sync();
+        if (in) keys[kept + mbcnt(who)] = k;
+        kept += (uint32_t)__popcll(who);
+      }
       wave_sync();
-      if (in)
-        keys[kept + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u))] = k;
-      kept += (uint32_t)__popcll(who);
+      count = kept;
     }
-    wave_sync();
-    count = kept > 64u ? keep_largest(keys, kept, N) : kept;
+    if (count > 64u) count = keep_largest(keys, count, N);
     if (lane == 0) s_count[wave] = count;
   }
   __syncthreads();
@@ -599,7 +642,7 @@ __global__ __launch_bounds__(kThreads, 5) void rows_kernel(Params p) {
     if (lane < count) s_list[before_me + lane] = keys[lane];
     __syncthreads();
   }
-  uint32_t before = 0;  // tokens of this part in front of given token tid
+  before = 0;  // tokens of this part in front of given token tid
   if (tid < T) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) before += s_before[w][tid];
@@ -626,33 +669,34 @@ __global__ __launch_bounds__(kThreads, 5) void rows_kernel(Params p) {
   if (TOP && tid >= all && tid < N) r.write_top(late.b, row, tid, 0);
 }
 
-// One wavefront joins the parts of a row. The alternatives are the keys no less than a bound that is
-// found by halving the range of keys until N to N + 4 of them are above it.
-template <int DT, bool CAP, int PER>
+// One wavefront joins the parts of a row. The alternatives are the keys no less than a bound that is found by halving
+// a range of keys until N to N + 4 of them are above it.
+template <int DT, bool CAP, bool TOP, int PER>
 __global__ __launch_bounds__(64) void merge_kernel(Params p) {
   const oxs_logprobs& b = p.b;
   const uint32_t row = blockIdx.x, lane = threadIdx.x;
-  const uint32_t S = p.splits, T = b.tokens_per_row, N = b.top_n;
-  __shared__ uint64_t s_list[64];
+  const uint32_t S = p.splits, T = b.tokens_per_row, N = TOP ? b.top_n : 0u;
+  __shared__ uint64_t s_best[64];
   const size_t at = (size_t)row * S;
   float4 st = make_float4(neg_inf(), 0.0f, 0.0f, 0.0f);
   if (lane < S) st = p.stats[at + lane];
-  uint64_t k[PER];
-  if (N) {
+  uint64_t k[PER], floor = ~0ull;
+  if constexpr (TOP) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) k[i] = lane + 64u * i < S * N ? p.keys[at * N + lane + 64u * i] : 0;
+    // the ceil(N / S)-th key of each part: N keys at least are no less than the smallest of them
+    if (lane < S) floor = p.keys[(at + lane) * N + (N + S - 1u) / S - 1u];
   }
   uint32_t want = kNoToken;
-  float want_l = neg_inf();
-  if (lane < T) {
-    want = b.tokens[(size_t)row * (size_t)b.tokens_ld + lane];
-    want_l = present_logit<DT>(b, row, want);
-  }
-  const float inv = inverse_temperature(b, row), c = inv * kLog2e;
-  const float cap = b.logit_softcap, inv_cap = CAP ? 1.0f / cap : 0.0f;
+  if (lane < T) want = b.tokens[(size_t)row * (size_t)b.tokens_ld + lane];
+  const float want_l = present_logit<DT>(b, row, want);
+  const float inv = inverse_temperature(b, row), c = inv * kLog2e, cap = b.logit_softcap, inv_cap = CAP ? 1.0f / cap : 0.0f;
+  const auto y_of = [&](float l) {
+    if constexpr (CAP) return l == neg_inf() ? l : softcap_of(l, cap, inv_cap);
+    else return l;
+  };
   const float m = wave_max(st.x);
-  const float d = fmaxf((capped<CAP>(st.x, cap, inv_cap) - capped<CAP>(m, cap, inv_cap)) * c, kFloor);
-  const float f = st.x == neg_inf() ? 0.0f : exp2_fast(d);
+  const float d = fmaxf((y_of(st.x) - y_of(m)) * c, kFloor), f = exp2_fast(d);
   const Row r(b, inv, m, wave_sum(f * st.y), wave_sum(f * __builtin_fmaf(d, st.y, st.z)));
   if (lane == 0) r.write(b, row);
   uint32_t before = 0;
@@ -661,44 +705,52 @@ __global__ __launch_bounds__(64) void merge_kernel(Params p) {
     if (lane == j) before = n;
   }
   if (lane < T) r.write_token(b, row, lane, want_l, before);
-  if (!N) return;
-  uint64_t lo = 1, hi = ~0ull;  // keys >= lo are enough (or all there are); fewer than N are >= hi
-  uint32_t n = 0;
+  if constexpr (TOP) {
+    uint64_t best = k[0];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) n += (uint32_t)__popcll(__ballot(k[i] >= lo));
-  for (int step = 0; step < 64 && n > N + 4u; ++step) {
-    const uint64_t mid = lo + (hi - lo) / 2u;
-    uint32_t some = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) some += (uint32_t)__popcll(__ballot(k[i] >= mid));
-    if (some >= N) {
-      lo = mid;
-      n = some;
-    } else {
-      hi = mid;
+    for (int i = 1; i < PER; ++i) best = k[i] > best ? k[i] : best;
+    for (int o = 32; o > 0; o >>= 1) {
+      const uint64_t x = __shfl_xor((unsigned long long)best, o), y = __shfl_xor((unsigned long long)floor, o);
+      best = x > best ? x : best;
+      floor = y < floor ? y : floor;
     }
-  }
-  uint32_t all = 0;  // n of them: at most N + 4 <= 64, as keys differ
+    uint64_t lo = floor ? floor : 1u, hi = best + 1u;  // keys >= lo are enough (or all there are); fewer than N are >= hi
+    uint32_t n = 0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const bool in = k[i] >= lo;
-    const uint64_t who = __ballot(in);
-    const uint32_t to =
-        all + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
-    if (in && to < 64u) s_list[to] = k[i];
-    all += (uint32_t)__popcll(who);
+    for (int i = 0; i < PER; ++i) n += (uint32_t)__popcll(__ballot(k[i] >= lo));
+    for (int step = 0; step < 64 && n > N + 4u; ++step) {
+      const uint64_t mid = lo + (hi - lo) / 2u;
+      uint32_t some = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) some += (uint32_t)__popcll(__ballot(k[i] >= mid));
+      if (some >= N) {
+        lo = mid;
+        n = some;
+      } else {
+        hi = mid;
+      }
+    }
+    uint32_t all = 0;  // n of them: at most N + 4 <= 64, as keys differ
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool in = k[i] >= lo;
+      const uint64_t who = __ballot(in);
+      const uint32_t to = all + mbcnt(who);
+      if (in && to < 64u) s_best[to] = k[i];
+      all += (uint32_t)__popcll(who);
+    }
+    all = min(all, 64u);
+    wave_sync();
+    uint32_t place = kNoToken;
+    uint64_t mine = 0;
+    if (lane < all) {
+      mine = s_best[lane];
+      place = 0;
+      for (uint32_t i = 0; i < all; ++i) place += s_best[i] > mine ? 1u : 0u;
+    }
+    if (place < N) r.write_top(b, row, place, mine);
+    if (lane >= all && lane < N) r.write_top(b, row, lane, 0);
   }
-  all = min(all, 64u);
-  __syncthreads();
-  uint32_t place = kNoToken;
-  uint64_t mine = 0;
-  if (lane < all) {
-    mine = s_list[lane];
-    place = 0;
-    for (uint32_t i = 0; i < all; ++i) place += s_list[i] > mine ? 1u : 0u;
-  }
-  if (place < N) r.write_top(b, row, place, mine);
-  if (lane >= all && lane < N) r.write_top(b, row, lane, 0);
 }
 
 template <int DT, bool CAP>
@@ -706,11 +758,11 @@ static void launch(Params& p, hipStream_t st) {
   const oxs_logprobs& b = p.b;
   // Tiles of 8192 logits (32 per thread), or of 2048 where those would leave CUs without a workgroup.
   const auto tiles_of = [&](uint32_t tile) { return (b.vocab + 7u + tile - 1u) / tile; };
-  const bool small = (uint64_t)b.rows * tiles_of(kThreads * 32) < 256u;
-  const uint32_t tiles = tiles_of(kThreads * (small ? 8 : 32));
+  const bool small = (uint64_t)b.rows * tiles_of(kThreads * LP_E) < 256u;
+  const uint32_t tiles = tiles_of(kThreads * (small ? 8 : LP_E));
   uint32_t splits = 1;
-  if (b.rows < 512u) {
-    splits = min(min(tiles, kMaxSplits), (1024u + b.rows - 1u) / b.rows);
+  if (b.rows < LP_ROWS) {
+    splits = min(min(tiles, kMaxSplits), (LP_TARGET + b.rows - 1u) / b.rows);
     if (b.top_n) splits = min(splits, kMergeKeys / b.top_n);
   }
   p.tiles = (tiles + splits - 1u) / splits;
@@ -728,11 +780,12 @@ static void launch(Params& p, hipStream_t st) {
     else by_top(e, std::false_type{});
   };
   if (small) by_mask(std::integral_constant<int, 8>{});
-  else by_mask(std::integral_constant<int, 32>{});
+  else by_mask(std::integral_constant<int, LP_E>{});
   if (p.splits == 1u) return;
   const auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(b.rows), dim3(64), 0, st, p); };
-  if (p.splits * b.top_n <= 5u * 64u) join(merge_kernel<DT, CAP, 5>);
-  else join(merge_kernel<DT, CAP, 20>);
+  if (b.top_n == 0u) join(merge_kernel<DT, CAP, false, 1>);
+  else if (p.splits * b.top_n <= 5u * 64u) join(merge_kernel<DT, CAP, true, 5>);
+  else join(merge_kernel<DT, CAP, true, 20>);
 }
 
 }  // namespace oxs_lp

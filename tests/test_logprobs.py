@@ -471,6 +471,22 @@ def test_graphs_streams_and_repeats(torch_gpu):
 
 
 @pytest.mark.gpu
+def test_one_workspace_for_calls_of_all_sizes(torch_gpu):
+    # rows split over workgroups in different ways, one call after the other on one workspace
+    from oxide_sampler import TokenLogprobs
+    lp, rng = TokenLogprobs(), np.random.default_rng(12)
+    for rows, V, dtype, T, top in ((1, 262147, "f32", 3, 32), (300, 9001, "bf16", 1, 4), (2, 40000, "f32", 64, 0),
+                                   (1, 70, "f32", 2, 8), (511, 3000, "f32", 1, 1), (33, 33000, "bf16", 2, 20),
+                                   (1, 262147, "bf16", 1, 3)):
+        x = wl.zipf_prior_logits(rng, min(rows, 3), V, 3.0)
+        x = np.ascontiguousarray(x[np.arange(rows) % len(x)])
+        x = bf16(x) if dtype == "bf16" else x
+        tokens = some_tokens(x, T, rng)
+        check(run(torch_gpu, x, tokens, top, dtype=dtype, lp=lp), reference(x, tokens, top), V,
+              what=f"rows={rows} V={V}")
+
+
+@pytest.mark.gpu
 def test_python_refusals(torch_gpu):
     from oxide_sampler import TokenLogprobs
     t = torch_gpu
