@@ -17,18 +17,6 @@
 
 #include "../../include/oxide_sampler.h"
 
-#ifndef LP_E
-#define LP_E 16
-#endif
-#ifndef LP_TARGET
-#define LP_TARGET 1024u
-#endif
-#ifndef LP_ROWS
-#define LP_ROWS 512u
-#endif
-#ifndef LP_OCC
-#define LP_OCC 5
-#endif
 namespace oxs_lp {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -42,12 +30,9 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.693147180559945309417f;
 // 2^-256 is 0 in 32 bits: a difference below this (or NaN, of two infinities) adds nothing
 constexpr float kFloor = -256.0f;
-#ifndef LP_SPLITS
-#define LP_SPLITS 64
-#endif
-constexpr uint32_t kMaxSplits = LP_SPLITS;      // parts of a row
+constexpr uint32_t kMaxSplits = 64;      // parts of a row
 constexpr uint32_t kMaxParts = 4096;     // rows * parts of a call that splits its rows
-constexpr uint32_t kMergeKeys = 20 * 64; // parts * top_n of a split row
+constexpr uint32_t kMergeKeys = 10 * 64; // parts * top_n of a split row
 constexpr uint32_t kRoom = OXS_LOGPROBS_MAX_TOP + 512;  // candidates of a wavefront: those kept, and 64 lanes' next 8
 
 struct Params {
@@ -706,15 +691,13 @@ __global__ __launch_bounds__(64) void merge_kernel(Params p) {
   }
   if (lane < T) r.write_token(b, row, lane, want_l, before);
   if constexpr (TOP) {
-    uint64_t best = k[0];
+    uint32_t best = (uint32_t)(k[0] >> 32);
 #pragma unroll
-    for (int i = 1; i < PER; ++i) best = k[i] > best ? k[i] : best;
-    for (int o = 32; o > 0; o >>= 1) {
-      const uint64_t x = __shfl_xor((unsigned long long)best, o), y = __shfl_xor((unsigned long long)floor, o);
-      best = x > best ? x : best;
-      floor = y < floor ? y : floor;
-    }
-    uint64_t lo = floor ? floor : 1u, hi = best + 1u;  // keys >= lo are enough (or all there are); fewer than N are >= hi
+    for (int i = 1; i < PER; ++i) best = max(best, (uint32_t)(k[i] >> 32));
+    best = wave_reduce(best, 0u, [](uint32_t x, uint32_t y) { return max(x, y); });
+    const uint32_t low = wave_reduce((uint32_t)(floor >> 32), ~0u, [](uint32_t x, uint32_t y) { return min(x, y); });
+    // keys >= lo are enough (or all there are); fewer than N are >= hi
+    uint64_t lo = low ? (uint64_t)low << 32 : 1u, hi = (uint64_t)(best + 1u) << 32;
     uint32_t n = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) n += (uint32_t)__popcll(__ballot(k[i] >= lo));
@@ -758,11 +741,11 @@ static void launch(Params& p, hipStream_t st) {
   const oxs_logprobs& b = p.b;
   // Tiles of 8192 logits (32 per thread), or of 2048 where those would leave CUs without a workgroup.
   const auto tiles_of = [&](uint32_t tile) { return (b.vocab + 7u + tile - 1u) / tile; };
-  const bool small = (uint64_t)b.rows * tiles_of(kThreads * LP_E) < 256u;
-  const uint32_t tiles = tiles_of(kThreads * (small ? 8 : LP_E));
+  const bool small = (uint64_t)b.rows * tiles_of(kThreads * 32) < 256u;
+  const uint32_t tiles = tiles_of(kThreads * (small ? 8 : 32));
   uint32_t splits = 1;
-  if (b.rows < LP_ROWS) {
-    splits = min(min(tiles, kMaxSplits), (LP_TARGET + b.rows - 1u) / b.rows);
+  if (b.rows < 512u) {
+    splits = min(min(tiles, kMaxSplits), (1024u + b.rows - 1u) / b.rows);
     if (b.top_n) splits = min(splits, kMergeKeys / b.top_n);
   }
   p.tiles = (tiles + splits - 1u) / splits;
@@ -780,12 +763,12 @@ static void launch(Params& p, hipStream_t st) {
     else by_top(e, std::false_type{});
   };
   if (small) by_mask(std::integral_constant<int, 8>{});
-  else by_mask(std::integral_constant<int, LP_E>{});
+  else by_mask(std::integral_constant<int, 32>{});
   if (p.splits == 1u) return;
   const auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(b.rows), dim3(64), 0, st, p); };
   if (b.top_n == 0u) join(merge_kernel<DT, CAP, false, 1>);
   else if (p.splits * b.top_n <= 5u * 64u) join(merge_kernel<DT, CAP, true, 5>);
-  else join(merge_kernel<DT, CAP, true, 20>);
+  else join(merge_kernel<DT, CAP, true, 10>);
 }
 
 }  // namespace oxs_lp
