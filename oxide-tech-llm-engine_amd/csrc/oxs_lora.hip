@@ -17,6 +17,21 @@
 
 #include "../../include/oxide_sampler.h"
 
+#ifndef LORA_PER
+#define LORA_PER 256u
+#endif
+#ifndef LORA_MINROWS
+#define LORA_MINROWS 8u
+#endif
+#ifndef LORA_SMALL
+#define LORA_SMALL 64u
+#endif
+#ifndef LORA_SPF
+#define LORA_SPF 2
+#endif
+#ifndef LORA_SOCC
+#define LORA_SOCC 3
+#endif
 namespace oxs_lora {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -139,46 +154,99 @@ __device__ __forceinline__ Eight<DT> load_eight(const Element<DT>* p) {
   return e;
 }
 
-// One wavefront per (row, PER ranks): its lanes take eight values of x at a time.
+// Where a row stands when the rows of its window are ordered by adapter, and what the second kernel has to know of it.
+struct Place {
+  uint32_t row, slot, rank, unused;
+};
+constexpr uint32_t kWindow = 1024;  // rows that are ordered among each other
+
+__device__ __forceinline__ void place_row(const oxs_lora_batch& b, uint32_t row, uint32_t a,
+                                          uint32_t rank, Place* places) {
+  __shared__ uint32_t s_count[kWaves];
+  const uint32_t start = row - row % kWindow, n = min(b.batch - start, kWindow);
+  uint32_t before = 0;
+  for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
+    const uint32_t other = b.adapters[start + j];
+    before += other < a || (other == a && start + j < row) ? 1u : 0u;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o);
+  if ((threadIdx.x & 63u) == 0u) s_count[threadIdx.x >> 6] = before;
+  __syncthreads();
+  if (threadIdx.x == 0) places[start + s_count[0] + s_count[1] + s_count[2] + s_count[3]] = Place{row, a, rank, 0u};
+}
+
+// One wavefront per (row, PER ranks): its lanes take eight values of x at a time, the first kAhead times before the
+// row's adapter is known. The last workgroup of a row finds the row's place instead.
 template <int WT, int XT, int PER>
-__global__ __launch_bounds__(kThreads) void shrink_kernel(oxs_lora_table t, oxs_lora_batch b, uint32_t vec) {
+__global__ __launch_bounds__(kThreads) void shrink_kernel(oxs_lora_table t, oxs_lora_batch b, Place* places,
+                                                          uint32_t vec) {
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t row = blockIdx.x, r0 = (blockIdx.y * kWaves + wave) * PER;
-  const uint32_t a = b.adapters[row], rank = rank_of(t, a), all_blocks = rank_blocks(t.max_rank);
-  if (r0 >= rank_blocks(rank) * kBlock) return;
+  const uint32_t a = b.adapters[row];
+  if (blockIdx.y + 1u == gridDim.y) {
+    place_row(b, row, a, rank_of(t, a), places);
+    return;
+  }
+  constexpr uint32_t kAhead = XT == OXS_DTYPE_F32 ? 4 : 8, kStride = 512;
+  const Element<XT>* x = (const Element<XT>*)b.x + (size_t)row * (size_t)b.x_ld;
+  const uint32_t from = lane * 8u;
+  Eight<XT> first[kAhead];
+  if (vec) {
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; ++j) {
+      first[j] = Eight<XT>{};
+      if (from + j * kStride + 8u <= t.k) first[j] = load_eight<XT>(x + from + j * kStride);
+    }
+  }
+  const uint32_t rank = rank_of(t, a), all_blocks = rank_blocks(t.max_rank);
+  // With a rank per wavefront the weights are not waited for until the adapter's rank is known: a slot has room for
+  // max_rank whatever it holds.
+  if (PER == 1 ? a >= t.max_adapters : r0 >= rank_blocks(rank) * kBlock) return;
+  const float scale = t.scales[a];
   const uint32_t kp = padded_k(t.k);
   const Element<WT>* w = (const Element<WT>*)t.a + (size_t)a * a_elements(t) + (size_t)r0 * kp;
-  const Element<XT>* x = (const Element<XT>*)b.x + (size_t)row * (size_t)b.x_ld;
   float s[PER];
 #pragma unroll
   for (int p = 0; p < PER; ++p) s[p] = 0.0f;
-#pragma unroll 4
-  for (uint32_t i = lane * 8u; i < t.k; i += 512u) {
-    float xv[8];
-    if (vec && i + 8u <= t.k) {
-      const Eight<XT> e = load_eight<XT>(x + i);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) xv[j] = e[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) xv[j] = i + j < t.k ? widen<XT>(x[i + j]) : 0.0f;
-    }
+  uint32_t i = from;
+  const auto add = [&](const float (&xv)[8]) {
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const Eight<WT> e = load_eight<WT>(w + (size_t)p * kp + i);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[p] = __builtin_fmaf(e[j], xv[j], s[p]);
     }
+  };
+  const auto add_eight = [&](const Eight<XT>& e) {
+    float xv[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) xv[j] = e[j];
+    add(xv);
+  };
+  if (vec) {
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; ++j, i += kStride) {
+      if (i + 8u > t.k) break;
+      add_eight(first[j]);
+    }
+#pragma unroll 4
+    for (; i + 8u <= t.k; i += kStride) add_eight(load_eight<XT>(x + i));
   }
-  const float scale = t.scales[a];
+  for (; i < t.k; i += kStride) {
+    float xv[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) xv[j] = i + j < t.k ? widen<XT>(x[i + j]) : 0.0f;
+    add(xv);
+  }
 #pragma unroll
   for (int p = 0; p < PER; ++p) {
     float v = s[p];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
     // ranks past the adapter's, up to the block's end, are zero
-    if (lane == 0) store_value(b.workspace, row, all_blocks, r0 + p, r0 + p < rank ? v * scale : 0.0f);
+    if (lane == 0 && r0 + p < rank_blocks(rank) * kBlock) store_value(b.workspace, row, all_blocks, r0 + p, r0 + p < rank ? v * scale : 0.0f);
   }
 }
 
@@ -236,24 +304,23 @@ struct Cursor {
   }
 };
 
-// One wavefront: 32 rows x 32 TT outputs (lane n: outputs TT n .. TT n + TT - 1). The rows are the first operand, the
-// outputs the second, so a register holds one row's 32 TT outputs side by side over 32 lanes. Each adapter's product
-// is computed for all 32 rows and taken for its own.
-// The weights of the next PF (adapter, rank block) pairs are on their way while one is worked on.
-template <int WT, int YT, int TT, int PF>
-__global__ __launch_bounds__(kThreads, 2) void expand_kernel(oxs_lora_table t, oxs_lora_batch b, uint32_t row_tiles,
-                                                             uint32_t col_tiles, uint32_t vec) {
+// One wavefront: `rows` <= 32 rows (in order of adapter; at most 8 with RR = 4, where only the first four registers of
+// a tile hold any) x 32 TT outputs (lane n: outputs TT n .. TT n + TT - 1); a
+// workgroup: the same rows and kWaves ranges of outputs side by side. The rows are the first operand, the outputs the
+// second, so a register holds one row's 32 TT outputs side by side over 32 lanes. Each adapter's product is computed
+// for all of the rows and taken for its own.
+// The operands of the next PF (adapter, rank block) pairs are on their way while one is worked on.
+template <int WT, int YT, int TT, int PF, int RR>
+__global__ __launch_bounds__(kThreads, RR == 4 ? LORA_SOCC : 2) void expand_kernel(oxs_lora_table t, oxs_lora_batch b, const Place* places,
+                                                             uint32_t rows, uint32_t col_groups, uint32_t vec) {
   const uint32_t lane = threadIdx.x & 63u, n = lane & 31u, g = lane >> 5;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t id = blockIdx.x * kWaves + wave;
-  const uint32_t col = id / row_tiles, row0 = (id - col * row_tiles) * kRows;
-  if (col >= col_tiles) return;
-  const uint32_t my_row = min(row0 + n, b.batch - 1u);
-  uint32_t ids = b.adapters[my_row];
-  if (row0 + n >= b.batch) ids = OXS_LORA_NONE;
-  const uint32_t ranks = rank_of(t, ids);
-  const uint32_t live = (uint32_t)__ballot(ranks != 0u);
-  if (live == 0u) return;
+  const uint32_t row_tile = blockIdx.x / col_groups;
+  const uint32_t col = (blockIdx.x - row_tile * col_groups) * kWaves + wave;
+  Place my = {0u, OXS_LORA_NONE, 0u, 0u};
+  if (n < rows && row_tile * rows + n < b.batch) my = places[row_tile * rows + n];
+  const uint32_t live = (uint32_t)__ballot(my.rank != 0u);
+  if (live == 0u || col * 32u * TT >= t.m) return;
   const uint32_t all_blocks = rank_blocks(t.max_rank);
   constexpr uint32_t kPieces = kBlock * kGroup;  // elements of a group's rank block
   constexpr uint32_t kPerGroup = kGroup / (32u * TT);
@@ -262,12 +329,12 @@ __global__ __launch_bounds__(kThreads, 2) void expand_kernel(oxs_lora_table t, o
   const uint32_t in_group = (col % kPerGroup) * 32u * TT + TT * n;
   const Element<WT>* wb = (const Element<WT>*)t.b + (size_t)(col / kPerGroup) * all_blocks * kPieces +
                           (g * 4u + in_group % 4u) * 256u + (in_group / 4u) * 8u;
-  const uint16_t* vb = (const uint16_t*)b.workspace + (size_t)my_row * all_blocks * (kValueBytes / 2) + g * 8u;
+  const uint16_t* vb = (const uint16_t*)b.workspace + (size_t)my.row * all_blocks * (kValueBytes / 2) + g * 8u;
 
   Cursor ahead;
   ahead.rest = live;
   ahead.slot = ahead.rank = 0;
-  ahead.adapter(ids, ranks);
+  ahead.adapter(my.slot, my.rank);
   Eight<WT> w[PF][TT];
   Eight<OXS_DTYPE_BF16> v[PF][kPlanes];
   uint32_t same[PF];
@@ -276,14 +343,14 @@ __global__ __launch_bounds__(kThreads, 2) void expand_kernel(oxs_lora_table t, o
     const bool in = g == 0u || ahead.block * kBlock + 8u < ahead.rank;  // this half holds a rank
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
+      w[i][tt] = Eight<WT>{};
       if (in) w[i][tt] = load_eight<WT>(p + tt * 256u);
-      else w[i][tt] = Eight<WT>{};
     }
 #pragma unroll
     for (int q = 0; q < (int)kPlanes; ++q)
       v[i][q] = load_eight<OXS_DTYPE_BF16>(vb + ahead.block * (kValueBytes / 2) + q * kBlock);
     same[i] = ahead.same;
-    ahead.next(ids, ranks);
+    ahead.next(my.slot, my.rank);
   };
 #pragma unroll
   for (int i = 0; i < PF; ++i) fetch(i);
@@ -291,27 +358,36 @@ __global__ __launch_bounds__(kThreads, 2) void expand_kernel(oxs_lora_table t, o
   // y, where a row has an adapter
   const uint32_t mine = live >> (4u * g);  // bit 8 (r / 4) + r % 4: register r's row
   using YE = Element<YT>;
-  YE* y = (YE*)b.y + (size_t)row0 * (size_t)b.y_ld + out0;
-  const bool whole = vec && out0 + TT <= t.m;
-  YE old[16][TT];
+  struct alignas(TT * sizeof(YE)) Vec {
+    YE e[TT];
+  };
+  const auto y_at = [&](int r) {
+    const uint32_t row = (uint32_t)__shfl((int)my.row, (int)out_row(r, g));
+    return (YE*)b.y + (size_t)row * (size_t)b.y_ld + out0;
+  };
+  const bool whole = vec != 0u && (uint64_t)(col + 1u) * 32u * TT <= t.m;
+  Vec old[RR];
+  if (whole) {
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    if (!((mine >> (8 * (r / 4) + r % 4)) & 1u)) continue;
-    const YE* p = y + (size_t)out_row(r, g) * (size_t)b.y_ld;
-    if (whole) {
-      struct alignas(TT * sizeof(YE)) Vec { YE e[TT]; };
-      const Vec q = *(const Vec*)p;
+    for (int r = 0; r < RR; ++r) {
+      const YE* p = y_at(r);
+      if ((mine >> (8 * (r / 4) + r % 4)) & 1u) old[r] = *(const Vec*)p;
+    }
+  } else {
 #pragma unroll
-      for (int tt = 0; tt < TT; ++tt) old[r][tt] = q.e[tt];
-    } else {
+    for (int r = 0; r < RR; ++r) {
+      const YE* p = y_at(r);
 #pragma unroll
-      for (int tt = 0; tt < TT; ++tt) old[r][tt] = out0 + tt < t.m ? p[tt] : 0;
+      for (int tt = 0; tt < TT; ++tt)
+        if (((mine >> (8 * (r / 4) + r % 4)) & 1u) && out0 + tt < t.m) old[r].e[tt] = p[tt];
     }
   }
 
-  f32x16 acc[TT];
+  float acc[TT][RR];
 #pragma unroll
-  for (int tt = 0; tt < TT; ++tt) acc[tt] = (f32x16){};
+  for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+    for (int r = 0; r < RR; ++r) acc[tt][r] = 0.0f;
   do {
 #pragma unroll
     for (int i = 0; i < PF; ++i) {
@@ -324,17 +400,22 @@ __global__ __launch_bounds__(kThreads, 2) void expand_kernel(oxs_lora_table t, o
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
           const Parts<WT> wp(w[i][tt]);
-          f32x16 d = s == live ? acc[tt] : (f32x16){};
+          f32x16 d = {};
+          if (RR == 16 && s == live) {  // one adapter for all: onto the sum
+#pragma unroll
+            for (int r = 0; r < RR; ++r) d[r] = acc[tt][r];
+          }
 #pragma unroll
           for (int sum = 2; sum >= 0; --sum)  // the small products first
 #pragma unroll
             for (int q = 0; q < Parts<WT>::N; ++q)
               if (q <= sum) d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vp[sum - q], wp.p[q], d, 0, 0, 0);
-          if (s == live) {
-            acc[tt] = d;
+          if (RR == 16 && s == live) {
+#pragma unroll
+            for (int r = 0; r < RR; ++r) acc[tt][r] = d[r];
           } else {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[tt][r] += (bits >> (8 * (r / 4) + r % 4)) & 1u ? d[r] : 0.0f;
+            for (int r = 0; r < RR; ++r) acc[tt][r] += (bits >> (8 * (r / 4) + r % 4)) & 1u ? d[r] : 0.0f;
           }
         }
       }
@@ -342,27 +423,35 @@ __global__ __launch_bounds__(kThreads, 2) void expand_kernel(oxs_lora_table t, o
     }
   } while (same[0]);
 
+  const auto sum = [&](int r) {
+    Vec z;
+    if constexpr (YT == OXS_DTYPE_BF16 && TT % 2 == 0) {
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    if (!((mine >> (8 * (r / 4) + r % 4)) & 1u)) continue;
-    YE* p = y + (size_t)out_row(r, g) * (size_t)b.y_ld;
-    YE out[TT];
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-      const float z = widen<YT>(old[r][tt]) + acc[tt][r];
-      if constexpr (YT == OXS_DTYPE_F32) out[tt] = __float_as_uint(z);
-      else out[tt] = (uint16_t)(narrow2(z, 0.0f) & 0xffffu);
-    }
-    if (whole) {
-      struct alignas(TT * sizeof(YE)) Vec { YE e[TT]; };
-      Vec q;
-#pragma unroll
-      for (int tt = 0; tt < TT; ++tt) q.e[tt] = out[tt];
-      *(Vec*)p = q;
+      for (int tt = 0; tt < TT; tt += 2) {
+        const uint32_t pair = narrow2(widen<YT>(old[r].e[tt]) + acc[tt][r], widen<YT>(old[r].e[tt + 1]) + acc[tt + 1][r]);
+        z.e[tt] = (YE)pair;
+        z.e[tt + 1] = (YE)(pair >> 16);
+      }
     } else {
 #pragma unroll
+      for (int tt = 0; tt < TT; ++tt) z.e[tt] = __float_as_uint(widen<YT>(old[r].e[tt]) + acc[tt][r]);
+    }
+    return z;
+  };
+  if (whole) {
+#pragma unroll
+    for (int r = 0; r < RR; ++r) {
+      YE* p = y_at(r);
+      if ((mine >> (8 * (r / 4) + r % 4)) & 1u) *(Vec*)p = sum(r);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < RR; ++r) {
+      YE* p = y_at(r);
+      const Vec z = sum(r);
+#pragma unroll
       for (int tt = 0; tt < TT; ++tt)
-        if (out0 + tt < t.m) p[tt] = out[tt];
+        if (((mine >> (8 * (r / 4) + r % 4)) & 1u) && out0 + tt < t.m) p[tt] = z.e[tt];
     }
   }
 }
@@ -427,7 +516,7 @@ extern "C" int oxs_lora_load(const oxs_lora_table* table, uint32_t slot, const v
 extern "C" size_t oxs_lora_workspace_bytes(const oxs_lora_table* table, uint32_t batch) {
   using namespace oxs_lora;
   if (!sizes_ok(table) || batch > 65536u) return 0;
-  return (size_t)(batch ? batch : 1u) * rank_blocks(table->max_rank) * kValueBytes;
+  return (size_t)(batch ? batch : 1u) * (rank_blocks(table->max_rank) * kValueBytes + sizeof(Place));
 }
 
 extern "C" int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* batch, void* stream) {
@@ -445,8 +534,8 @@ extern "C" int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* b
     return OXS_ERR_INVALID_ARGUMENT;
   if ((uint64_t)b.batch * t.m > (1ull << 31)) return OXS_ERR_LIMITS;
   const hipStream_t st = (hipStream_t)stream;
-  const uint32_t row_tiles = (b.batch + kRows - 1u) / kRows;
-  const uint32_t ranks = rank_blocks(t.max_rank) * kBlock;
+  const uint32_t blocks = rank_blocks(t.max_rank);
+  Place* places = (Place*)((char*)b.workspace + (size_t)b.batch * blocks * kValueBytes);
   const auto even = [](const void* p, int64_t ld, uint32_t es, uint32_t to) {
     return aligned(p, to) && ((uint64_t)ld * es) % to == 0;
   };
@@ -455,14 +544,26 @@ extern "C" int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* b
     by_values(b.x_dtype, [&](auto xt) {
       constexpr int XT = decltype(xt)::value;
       const uint32_t vec = even(b.x, b.x_ld, size_of(XT), 16) ? 1u : 0u;
-      hipLaunchKernelGGL((shrink_kernel<WT, XT, 1>), dim3(b.batch, ranks / kWaves), dim3(kThreads), 0, st, t, b, vec);
+      if ((uint64_t)b.batch * blocks >= LORA_PER)
+        hipLaunchKernelGGL((shrink_kernel<WT, XT, 4>), dim3(b.batch, blocks + 1u), dim3(kThreads), 0, st, t, b, places,
+                           vec);
+      else
+        hipLaunchKernelGGL((shrink_kernel<WT, XT, 1>), dim3(b.batch, blocks * 4u + 1u), dim3(kThreads), 0, st, t, b, places,
+                           vec);
     });
     by_values(b.y_dtype, [&](auto yt) {
-      constexpr int YT = decltype(yt)::value, TT = 2;
-      const uint32_t col_tiles = (t.m + 32u * TT - 1u) / (32u * TT);
+      constexpr int YT = decltype(yt)::value, TT = WT == OXS_DTYPE_F32 ? 2 : 4;
+      const uint32_t col_groups = (t.m + 32u * TT * kWaves - 1u) / (32u * TT * kWaves);
       const uint32_t vec = even(b.y, b.y_ld, size_of(YT), TT * size_of(YT)) ? 1u : 0u;
-      hipLaunchKernelGGL((expand_kernel<WT, YT, TT, 4>), dim3((row_tiles * col_tiles + kWaves - 1u) / kWaves),
-                         dim3(kThreads), 0, st, t, b, row_tiles, col_tiles, vec);
+      uint32_t rows = kRows;
+      if (b.batch <= LORA_SMALL) rows = LORA_MINROWS;
+      const uint32_t row_tiles = (b.batch + rows - 1u) / rows;
+      const auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(row_tiles * col_groups), dim3(kThreads), 0, st, t, b, places, rows, col_groups,
+                           vec);
+      };
+      if (rows <= 8u) go(expand_kernel<WT, YT, TT, LORA_SPF, 4>);
+      else go(expand_kernel<WT, YT, TT, 2, 16>);
     });
   });
   return launched();
