@@ -17,21 +17,6 @@
 
 #include "../../include/oxide_sampler.h"
 
-#ifndef LORA_PER
-#define LORA_PER 256u
-#endif
-#ifndef LORA_MINROWS
-#define LORA_MINROWS 8u
-#endif
-#ifndef LORA_SMALL
-#define LORA_SMALL 64u
-#endif
-#ifndef LORA_SPF
-#define LORA_SPF 2
-#endif
-#ifndef LORA_SOCC
-#define LORA_SOCC 3
-#endif
 namespace oxs_lora {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -44,6 +29,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr uint32_t kRows = 32;        // rows of a matrix tile
+constexpr uint32_t kFewRows = 48;     // batches that take tiles of 8
 constexpr uint32_t kGroup = 128;      // outputs of a group in the table
 constexpr uint32_t kBlock = 16;       // ranks of a block: the depth of a matrix instruction
 constexpr uint32_t kPlanes = 3;       // bf16 parts of a value of v
@@ -311,7 +297,7 @@ struct Cursor {
 // for all of the rows and taken for its own.
 // The operands of the next PF (adapter, rank block) pairs are on their way while one is worked on.
 template <int WT, int YT, int TT, int PF, int RR>
-__global__ __launch_bounds__(kThreads, RR == 4 ? LORA_SOCC : 2) void expand_kernel(oxs_lora_table t, oxs_lora_batch b, const Place* places,
+__global__ __launch_bounds__(kThreads, RR == 4 ? 3 : 2) void expand_kernel(oxs_lora_table t, oxs_lora_batch b, const Place* places,
                                                              uint32_t rows, uint32_t col_groups, uint32_t vec) {
   const uint32_t lane = threadIdx.x & 63u, n = lane & 31u, g = lane >> 5;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -544,7 +530,7 @@ extern "C" int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* b
     by_values(b.x_dtype, [&](auto xt) {
       constexpr int XT = decltype(xt)::value;
       const uint32_t vec = even(b.x, b.x_ld, size_of(XT), 16) ? 1u : 0u;
-      if ((uint64_t)b.batch * blocks >= LORA_PER)
+      if ((uint64_t)b.batch * blocks >= 256u)
         hipLaunchKernelGGL((shrink_kernel<WT, XT, 4>), dim3(b.batch, blocks + 1u), dim3(kThreads), 0, st, t, b, places,
                            vec);
       else
@@ -553,16 +539,17 @@ extern "C" int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* b
     });
     by_values(b.y_dtype, [&](auto yt) {
       constexpr int YT = decltype(yt)::value, TT = WT == OXS_DTYPE_F32 ? 2 : 4;
-      const uint32_t col_groups = (t.m + 32u * TT * kWaves - 1u) / (32u * TT * kWaves);
       const uint32_t vec = even(b.y, b.y_ld, size_of(YT), TT * size_of(YT)) ? 1u : 0u;
-      uint32_t rows = kRows;
-      if (b.batch <= LORA_SMALL) rows = LORA_MINROWS;
+      const uint32_t rows = b.batch <= kFewRows ? 8u : kRows;
       const uint32_t row_tiles = (b.batch + rows - 1u) / rows;
+      uint32_t col_groups = (t.m + 32u * TT * kWaves - 1u) / (32u * TT * kWaves);
+      // a multiple of 8: the workgroups of a range of outputs are all on one XCD, whose L2 then holds its weights
+      if (row_tiles > 1u) col_groups = (col_groups + 7u) / 8u * 8u;
       const auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(row_tiles * col_groups), dim3(kThreads), 0, st, t, b, places, rows, col_groups,
                            vec);
       };
-      if (rows <= 8u) go(expand_kernel<WT, YT, TT, LORA_SPF, 4>);
+      if (rows <= 8u) go(expand_kernel<WT, YT, TT, 2, 4>);
       else go(expand_kernel<WT, YT, TT, 2, 16>);
     });
   });
