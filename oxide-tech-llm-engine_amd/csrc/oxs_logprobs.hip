@@ -111,6 +111,9 @@ __device__ __forceinline__ void wave_sync() {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// 1 / cap, finite for the smallest caps too (0 times it is 0)
+__device__ __forceinline__ float inverse_cap(float cap) { return fminf(1.0f / cap, 3.402823466e38f); }
+
 // cap tanh(l / cap), to about 3 units in the last place: (1 - e) / (1 + e) with
 // e = e^(-2|x|), which cancels near 0, and the series up to x^9 below 1/4
 // (the next term is 0.009 x^10 <= 2^-26 of the value there).
@@ -124,12 +127,6 @@ __device__ __forceinline__ float softcap_of(float l, float cap, float inv_cap) {
   p = __builtin_fmaf(w, p, -1.0f / 3.0f);
   const float near = __builtin_fmaf(a * w, p, a);
   return cap * __builtin_copysignf(a < 0.25f ? near : far, x);
-}
-
-template <bool CAP>
-__device__ __forceinline__ float capped(float l, float cap, float inv_cap) {
-  if constexpr (CAP) return softcap_of(l, cap, inv_cap);
-  return l;
 }
 
 // 1 / T of a row, as the decode step takes it: greedy rows stay as they are.
@@ -163,7 +160,7 @@ struct Row {
   bool empty, over;
   __device__ __forceinline__ Row(const oxs_logprobs& b, float inv_, float m_, float s_, float t_)
       : m(m_), s(s_), t(t_), cap(b.logit_softcap), inv(inv_) {
-    inv_cap = 1.0f / cap;
+    inv_cap = inverse_cap(cap);
     empty = m == neg_inf();
     y_m = y_of(m);
     over = y_m == __builtin_inff();
@@ -346,7 +343,7 @@ __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
   const uint32_t skip = ((uint32_t)(uintptr_t)base & 15u) / kSize;
   const uint32_t* mask = MASK ? b.allowed_mask + (size_t)row * (size_t)b.mask_ld : nullptr;
   const float inv = inverse_temperature(b, row), c = inv * kLog2e;
-  const float cap = b.logit_softcap, inv_cap = CAP ? 1.0f / cap : 0.0f;
+  const float cap = b.logit_softcap, inv_cap = CAP ? inverse_cap(cap) : 0.0f;
   const auto y_of = [&](float l) {
     if constexpr (CAP) return l == neg_inf() ? l : softcap_of(l, cap, inv_cap);
     else return l;
@@ -683,7 +680,7 @@ __global__ __launch_bounds__(64) void merge_kernel(Params p) {
   uint32_t want = kNoToken;
   if (lane < T) want = b.tokens[(size_t)row * (size_t)b.tokens_ld + lane];
   const float want_l = present_logit<DT>(b, row, want);
-  const float inv = inverse_temperature(b, row), c = inv * kLog2e, cap = b.logit_softcap, inv_cap = CAP ? 1.0f / cap : 0.0f;
+  const float inv = inverse_temperature(b, row), c = inv * kLog2e, cap = b.logit_softcap, inv_cap = CAP ? inverse_cap(cap) : 0.0f;
   const auto y_of = [&](float l) {
     if constexpr (CAP) return l == neg_inf() ? l : softcap_of(l, cap, inv_cap);
     else return l;
@@ -816,10 +813,11 @@ extern "C" int oxs_token_logprobs(const oxs_logprobs* lp, void* stream) {
   if (b.workspace_bytes < oxs_logprobs_workspace_bytes()) return OXS_ERR_INVALID_ARGUMENT;
   oxs_lp::Params p{};
   p.b = b;
+  if (b.logit_softcap == __builtin_inff()) p.b.logit_softcap = 0.0f;  // what cap tanh(l / cap) tends to
   p.stats = (float4*)b.workspace;
   p.keys = (uint64_t*)(p.stats + oxs_lp::kMaxParts);
   p.counts = (uint32_t*)(p.keys + (size_t)oxs_lp::kMaxParts * OXS_LOGPROBS_MAX_TOP);
-  const bool cap = b.logit_softcap > 0.0f;
+  const bool cap = p.b.logit_softcap > 0.0f;
   const hipStream_t st = (hipStream_t)stream;
   if (b.logits_dtype == OXS_DTYPE_F32) {
     if (cap) oxs_lp::launch<OXS_DTYPE_F32, true>(p, st);

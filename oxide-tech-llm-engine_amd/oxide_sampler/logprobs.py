@@ -126,13 +126,10 @@ class TokenLogprobs:
 
     def compute(self, logits, tokens=None, *, top: int = 0, mask=None, temperatures=None, softcap: float = 0.0,
                 out=None, stream=None):
-        """`descriptor` and `launch` in one; returns the outputs. Outputs that
-        the call allocates belong to the current stream: with another `stream`
-        that is still at work, give `out`."""
-        call, outs = self.descriptor(logits, tokens, top=top, mask=mask, temperatures=temperatures, softcap=softcap,
-                                     out=out)
-        self.launch(call, stream)
-        if stream is not None:
-            for o in outs.values():
-                o.record_stream(stream)
+        """`descriptor` and `launch` in one; returns the outputs. With `stream`,
+        the outputs that the call allocates belong to that stream."""
+        with self.torch.cuda.stream(stream):
+            call, outs = self.descriptor(logits, tokens, top=top, mask=mask, temperatures=temperatures,
+                                         softcap=softcap, out=out)
+            self.launch(call, stream)
         return outs

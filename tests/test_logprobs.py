@@ -385,6 +385,34 @@ def test_temperatures_at_the_edges(torch_gpu, temp):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,V", [(4, 1500), (3, 33000), (600, 900)])
+def test_softcaps_at_the_edges(torch_gpu, rows, V, dtype):
+    rng = np.random.default_rng(V)
+    x = bf16(wl.zipf_prior_logits(rng, rows, V, 3.0))
+    x[:, ::7] = 0.0
+    x[0, 3:] = NINF
+    tokens = some_tokens(x, 4, rng)
+    got = run(torch_gpu, x, tokens, 5, softcap=1e-40, dtype=dtype)  # every logit becomes 0 to 40 places
+    check(got, reference(x, tokens, 5, softcap=1e-40), V)
+    plain = run(torch_gpu, x, tokens, 5, dtype=dtype)
+    got = run(torch_gpu, x, tokens, 5, softcap=np.inf, dtype=dtype)  # tends to no cap
+    for name in plain:
+        np.testing.assert_array_equal(got[name], plain[name], err_msg=name)
+    # 1e30 is as good as none: the division, the series and the product round y by 4u |l| at most, and of a log
+    # probability's or the entropy's terms three hold a y
+    got, ref = run(torch_gpu, x, tokens, 5, softcap=1e30, dtype=dtype), reference(x, tokens, 5)
+    most = 12 * U * np.abs(x[np.isfinite(x)]).max()
+    tol = tolerances(ref, V)
+    for name, bound in (("logsumexp", tol["logsumexp"]), ("logprobs", tol["logprobs"][:, None])):
+        r = ref[name]
+        fin = np.isfinite(r)
+        np.testing.assert_array_equal(got[name][~fin], r[~fin].astype(np.float32))
+        off = np.abs(got[name][fin] - r[fin])
+        assert (off <= np.broadcast_to(bound, r.shape)[fin] + most + 6 * U * np.abs(r[fin])).all(), name
+
+
+@pytest.mark.gpu
 def test_only_the_asked_outputs_are_written(torch_gpu):
     from oxide_sampler import TokenLogprobs
     t = torch_gpu
