@@ -535,7 +535,7 @@ typedef struct oxs_logprobs {
   const uint32_t* allowed_mask; /* optional, as oxs_batch.allowed_mask */
   int64_t mask_ld;              /* as oxs_batch.mask_ld */
   const float* temperatures;    /* optional [rows] */
-  float logit_softcap;          /* as oxs_batch.logit_softcap */
+  float logit_softcap;          /* as oxs_batch.logit_softcap; +inf is none */
   uint32_t top_n;               /* alternatives per row, 0 to OXS_LOGPROBS_MAX_TOP */
   float* out_logprobs;      /* optional [rows][T] */
   uint32_t* out_ranks;      /* optional [rows][T] */
@@ -603,6 +603,9 @@ int oxs_lora_table_bytes(const oxs_lora_table* table, size_t* a_bytes, size_t* b
  * it at its next replay): a is [rank][a_ld] and b is [m][b_ld], device, of
  * the table's dtype, a_ld >= k and b_ld >= rank. rank 0 empties the slot (a
  * and b may be NULL). Must not overlap an oxs_lora_add on another stream.
+ * Returns OXS_ERR_INVALID_ARGUMENT for a slot or rank above the table's,
+ * missing or misaligned pointers, or leading dimensions that are too small
+ * (where there is more than one row), OXS_ERR_HIP if the launch fails.
  */
 int oxs_lora_load(const oxs_lora_table* table, uint32_t slot, const void* a, int64_t a_ld, const void* b,
                   int64_t b_ld, uint32_t rank, float scale, void* stream);
@@ -626,10 +629,13 @@ size_t oxs_lora_workspace_bytes(const oxs_lora_table* table, uint32_t batch);
 
 /*
  * y_b += B_a (s_a A_a x_b) for every row b with a loaded adapter a =
- * adapters[b]; a row whose slot is empty or >= max_adapters is neither read
- * nor written. Products are exact and sums are in 32 bits; the result is
- * added to y in 32 bits and rounded to y_dtype once. Rows may have any
- * adapters in any order; rows of one adapter that stand together share reads.
+ * adapters[b]; y of a row whose slot is empty or >= max_adapters is neither
+ * read nor written. Weights, x and A x enter their products with all of their
+ * bits (a weight of B or a value of A x beyond the largest bfloat16, 3.39e38,
+ * counts as infinite) and sums are in 32 bits; the result is added to y in 32
+ * bits and rounded to y_dtype once. Rows may have any adapters in any order;
+ * the rows of an adapter share its reads. Repeated calls give equal bits. y
+ * must not overlap the other arrays.
  * An infinity or NaN in one adapter's weights or one row's x reaches no row
  * but those of that adapter and that row. Asynchronous and stream ordered on
  * the current device; allocates nothing and issues only kernels. Returns

@@ -522,8 +522,8 @@ extern "C" int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* b
   const hipStream_t st = (hipStream_t)stream;
   const uint32_t blocks = rank_blocks(t.max_rank);
   Place* places = (Place*)((char*)b.workspace + (size_t)b.batch * blocks * kValueBytes);
-  const auto even = [](const void* p, int64_t ld, uint32_t es, uint32_t to) {
-    return aligned(p, to) && ((uint64_t)ld * es) % to == 0;
+  const auto even = [&](const void* p, int64_t ld, uint32_t es, uint32_t to) {
+    return aligned(p, to) && (b.batch == 1 || ((uint64_t)ld * es) % to == 0);
   };
   by_weights(t.dtype, [&](auto wt) {
     constexpr int WT = decltype(wt)::value;

@@ -57,6 +57,7 @@ class LoraAdapters:
         self.ranks = t.zeros(self.max_adapters, dtype=t.int32, device=self.device)
         self.scales = t.zeros(self.max_adapters, dtype=t.float32, device=self.device)
         self.workspace = t.empty(self._bytes, dtype=t.uint8, device=self.device)
+        t.cuda.current_stream(self.device).synchronize()  # the slots are empty for every stream
         self.table.a, self.table.b = self._a.data_ptr(), self._b.data_ptr()
         self.table.ranks, self.table.scales = self.ranks.data_ptr(), self.scales.data_ptr()
 

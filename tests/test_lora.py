@@ -202,6 +202,41 @@ def test_matches_the_definition(torch_gpu, batch, m, k, ranks, w, xd, yd, order)
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch,ranks,w", [(47, [16] * 5, "bf16"), (48, [8, 3], "f32"), (49, [16] * 5, "bf16"),
+                                           (1023, [4] * 3, "f16"), (1024, [16], "bf16"), (1025, [5, 16], "f32"),
+                                           (2100, [8, 0, 20], "bf16"), (3000, [2] * 100, "bf16")])
+@pytest.mark.parametrize("order", ["mixed", "packed", "falling"])
+def test_batches_around_the_kernels_own_sizes(torch_gpu, batch, ranks, w, order):
+    t = torch_gpu
+    m, k = 200, 40
+    x, y, ad, dt, g = make(t, batch, batch, m, k, ranks, w)
+    ids = t.randint(-1, len(ranks) + 1, (batch,), generator=g, device="cuda", dtype=t.int32)
+    if order != "mixed":
+        ids = ids.sort(descending=order == "falling").values
+    want, bound = reference(y, x, ids, ad)
+    table(t, m, k, ranks, ad, dt, batch).add(y, x, ids)
+    check(y, want, bound, f"{batch} {order}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k", [(50257, 895), (129, 4095), (6, 513)])
+@pytest.mark.parametrize("w", ["f32", "bf16", "f16"])
+def test_one_row_of_odd_sizes(torch_gpu, m, k, w):
+    t = torch_gpu
+    x, y, ad, dt, g = make(t, m, 1, m, k, [0, 31], w)
+    ids = t.ones(1, dtype=t.int32, device="cuda")
+    lora = table(t, m, k, [0, 31], ad, dt, 1)
+    for shift in (0, 1, 4):
+        yv = t.full((m + 8,), 7.0, device="cuda")
+        xv = t.full((k + 8,), float("nan"), device="cuda")
+        yv[shift:shift + m], xv[shift:shift + k] = y[0], x[0]
+        want, bound = reference(y, x, ids, ad)
+        lora.add(yv[shift:shift + m][None], xv[shift:shift + k][None], ids)
+        check(yv[shift:shift + m][None], want, bound, f"shift {shift}")
+        assert bool((yv[:shift] == 7).all()) and bool((yv[shift + m:] == 7).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("xd,yd,xpad,ypad,xshift,yshift", [("f32", "f32", 1, 3, 1, 1), ("bf16", "bf16", 5, 1, 3, 1),
                                                            ("f32", "f32", 4, 4, 0, 0), ("bf16", "f32", 8, 2, 8, 2),
                                                            ("f32", "bf16", 2, 8, 2, 4)])
