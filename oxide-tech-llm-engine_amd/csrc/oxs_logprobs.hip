@@ -295,19 +295,20 @@ struct Sums {
   // N more logits, of which none is 2^kSlack above ref
   template <int N, class Y>
   __device__ __forceinline__ void add(const float* v, float c, Y y) {
-    float s1 = 0.0f, t1 = 0.0f;
+    // two sums of their own first: a row's terms then pass N / 2 + V / (kThreads N) additions, not V / kThreads
+    float s0, s1, t0, t1;
 #pragma unroll
     for (int e = 0; e < N; e += 2) {
       const float q0 = fmaxf(__builtin_fmaf(y(v[e]), c, -rc), kFloor);
       const float q1 = fmaxf(__builtin_fmaf(y(v[e + 1]), c, -rc), kFloor);
       const float p0 = exp2_fast(q0), p1 = exp2_fast(q1);
-      s += p0;
-      s1 += p1;
-      t = __builtin_fmaf(q0, p0, t);
-      t1 = __builtin_fmaf(q1, p1, t1);
+      s0 = e ? s0 + p0 : p0;
+      s1 = e ? s1 + p1 : p1;
+      t0 = e ? __builtin_fmaf(q0, p0, t0) : q0 * p0;
+      t1 = e ? __builtin_fmaf(q1, p1, t1) : q1 * p1;
     }
-    s += s1;
-    t += t1;
+    s += s0 + s1;
+    t += t0 + t1;
   }
 };
 
@@ -395,7 +396,22 @@ __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
       }
     }
   };
+  // A wavefront's part of a group is 64 G tokens, whose mask is kWords words: all words of a tile come in one load
+  // (two for rows that do not begin on 16 bytes), lane g kWords + i holding the bits of group g from token 32 i on,
+  // and the lanes pass them on. Bits of tokens outside the row may be anything: those are -inf already.
+  constexpr uint32_t kWords = 2 * G;
+  uint32_t words[2] = {};
+  const auto fetch_mask = [&](uint32_t tile) {
+    if constexpr (MASK) {
+      const int32_t end = (int32_t)((V + 31u) / 32u) - 1;
+      const int32_t w = (int32_t)(tile * (kTile / 32u) + lane / kWords * (kThreads * G / 32u) + wave * kWords +
+                                  lane % kWords - (skip ? 1u : 0u));
+      words[0] = mask[min(max(w, 0), end)];
+      if (skip) words[1] = mask[min(w + 1, end)];
+    }
+  };
   u32x4 raw[NG];
+  fetch_mask(first);
   fetch(first, raw);
   if (want < V) {
     if constexpr (DT == OXS_DTYPE_F32) want_bits = *(const uint32_t*)(base + want * kSize);
@@ -414,22 +430,22 @@ __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
     const int32_t at = (int32_t)(tile * kTile + tid * G - skip);  // V <= 2^30
     const int64_t begin = (int64_t)tile * kTile - (int64_t)skip;  // of the tile
     float v[E];
-    const auto masked = [&](int g) {  // group g's logits that the mask leaves out become -inf
-      const uint32_t words = (V + 31u) / 32u;
-      const int32_t i = max(at + g * kThreads * G, 0);  // (before the row: -inf already; its bits are those from 0 on)
-      const int32_t d = i - (at + g * kThreads * G);
-      const uint32_t w = min((uint32_t)i >> 5, words - 1u);
-      uint32_t bits = mask[w] >> (i & 31);
-      if ((i & 31) > 32 - G && w + 1u < words) bits |= mask[w + 1u] << (32 - (i & 31));
-      bits <<= d;
+    uint32_t keep = 0;  // bit e: the mask allows element e
+    if constexpr (MASK) {
+      const uint32_t bits = __builtin_amdgcn_alignbit(words[1], words[0], 32u - skip);
 #pragma unroll
-      for (int e = 0; e < G; ++e)
-        if (!((bits >> e) & 1u)) v[g * G + e] = neg_inf();
-    };
+      for (int g = 0; g < NG; ++g) {
+        const uint32_t from = (uint32_t)__builtin_amdgcn_ds_bpermute((int)(g * kWords + lane * G / 32u) * 4, (int)bits);
+        keep |= ((from >> (lane * G % 32u)) & ((1u << G) - 1u)) << (g * G);
+      }
+    }
     u32x4 next[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) next[g] = raw[g];
-    if (tile + 1u < last) fetch(tile + 1u, next);
+    if (tile + 1u < last) {
+      fetch_mask(tile + 1u);
+      fetch(tile + 1u, next);
+    }
     const Sums before_tile = sums;
     float top = neg_inf();  // the thread's largest of the tile
     bool odd = false;
@@ -443,7 +459,10 @@ __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
       float x;
       if constexpr (MASK) {
 #pragma unroll
-        for (int g = e0 / G; g < (e0 + kStep) / G; ++g) masked(g);
+        for (int e = e0; e < e0 + kStep; ++e) {
+          const uint32_t in = (uint32_t)((int32_t)(keep << (31 - e)) >> 31);
+          v[e] = __uint_as_float((__float_as_uint(v[e]) & in) | (~in & 0xff800000u));
+        }
       }
       if constexpr (DT == OXS_DTYPE_BF16 && !MASK) x = largest_of_pairs(raw[e0 / G]);
       else x = largest_of<kStep>(v + e0);

@@ -374,6 +374,24 @@ def test_mask_bits_past_the_vocabulary_are_ignored(torch_gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,V", [(16, 1), (16, 30), (9, 33), (9, 2047), (9, 8200), (40, 32769), (600, 20001)])
+def test_masks_of_rows_on_every_boundary(torch_gpu, rows, V, dtype):
+    # odd strides: the rows begin on every element boundary of 16 bytes, and their masks' words on none of them
+    rng = np.random.default_rng(V)
+    x = bf16(rng.standard_normal((min(rows, 40), V)).astype(np.float32))[np.arange(rows) % min(rows, 40)]
+    m = rng.random((rows, V)) < rng.random((rows, 1))
+    m[0], m[-1] = True, False
+    m[1], m[2] = np.arange(V) == V - 1, np.arange(V) == 0
+    tokens = some_tokens(x, 3, rng)
+    for pad in (1 if V % 2 == 0 else 0, 8 - V % 8):
+        got = run(torch_gpu, x, tokens, 4, m, dtype=dtype, pad=pad)
+        check(got, reference(x, tokens, 4, m), V, what=f"pad {pad}")
+        got = run(torch_gpu, x, tokens, 0, m, dtype=dtype, pad=pad)
+        check(got, reference(x, tokens, 0, m), V, what=f"pad {pad}, no alternatives")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("temp", [1e-7, 1e-6, 2e-6, 1e-3, 50.0, float("inf"), float("nan"), -1.0])
 def test_temperatures_at_the_edges(torch_gpu, temp):
     rng = np.random.default_rng(3)
