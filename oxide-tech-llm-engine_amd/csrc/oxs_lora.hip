@@ -29,7 +29,6 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr uint32_t kRows = 32;        // rows of a matrix tile
-constexpr uint32_t kFewRows = 48;     // batches that take tiles of 8
 constexpr uint32_t kGroup = 128;      // outputs of a group in the table
 constexpr uint32_t kBlock = 16;       // ranks of a block: the depth of a matrix instruction
 constexpr uint32_t kPlanes = 3;       // bf16 parts of a value of v
@@ -140,6 +139,14 @@ __device__ __forceinline__ Eight<DT> load_eight(const Element<DT>* p) {
   return e;
 }
 
+// The same from memory aligned to its elements only.
+template <int DT>
+__device__ __forceinline__ Eight<DT> load_unaligned(const Element<DT>* p) {
+  Eight<DT> e;
+  __builtin_memcpy(&e, p, sizeof(e));
+  return e;
+}
+
 // Where a row stands when the rows of its window are ordered by adapter, and what the second kernel has to know of it.
 struct Place {
   uint32_t row, slot, rank, unused;
@@ -150,10 +157,14 @@ __device__ __forceinline__ void place_row(const oxs_lora_batch& b, uint32_t row,
                                           uint32_t rank, Place* places) {
   __shared__ uint32_t s_count[kWaves];
   const uint32_t start = row - row % kWindow, n = min(b.batch - start, kWindow);
+  uint32_t other[kWindow / kThreads];  // (all loads before the first is waited for)
+#pragma unroll
+  for (uint32_t i = 0; i < kWindow / kThreads; ++i) other[i] = b.adapters[start + min(threadIdx.x + i * kThreads, n - 1u)];
   uint32_t before = 0;
-  for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
-    const uint32_t other = b.adapters[start + j];
-    before += other < a || (other == a && start + j < row) ? 1u : 0u;
+#pragma unroll
+  for (uint32_t i = 0; i < kWindow / kThreads; ++i) {
+    const uint32_t j = threadIdx.x + i * kThreads;
+    before += j < n && (other[i] < a || (other[i] == a && start + j < row)) ? 1u : 0u;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o);
@@ -162,11 +173,28 @@ __device__ __forceinline__ void place_row(const oxs_lora_batch& b, uint32_t row,
   if (threadIdx.x == 0) places[start + s_count[0] + s_count[1] + s_count[2] + s_count[3]] = Place{row, a, rank, 0u};
 }
 
-// One wavefront per (row, PER ranks): its lanes take eight values of x at a time, the first kAhead times before the
-// row's adapter is known. The last workgroup of a row finds the row's place instead.
+// The sum over a wavefront's lanes, in every lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float plus_dpp(float x) {
+  const int from = __builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, ROWS, 0xf, false);
+  return x + __uint_as_float((uint32_t)from);
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  x = plus_dpp<0x111, 0xf>(x);  // lanes 1, 2, 4, 8 below in the row of 16
+  x = plus_dpp<0x112, 0xf>(x);
+  x = plus_dpp<0x114, 0xf>(x);
+  x = plus_dpp<0x118, 0xf>(x);
+  x = plus_dpp<0x142, 0xa>(x);  // the row before, into rows 1 and 3
+  x = plus_dpp<0x143, 0xc>(x);  // lane 31, into rows 2 and 3
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), 63));
+}
+
+// One wavefront per (row, PER ranks): its lanes take eight values of x at a time. The loads of kAhead times 512 values
+// are on their way together, those of the first x before the row's adapter is known; lanes past the end load what
+// others do, for nothing: a load behind a branch would be waited for on its own. The last workgroup of a row finds the
+// row's place instead.
 template <int WT, int XT, int PER>
-__global__ __launch_bounds__(kThreads) void shrink_kernel(oxs_lora_table t, oxs_lora_batch b, Place* places,
-                                                          uint32_t vec) {
+__global__ __launch_bounds__(kThreads) void shrink_kernel(oxs_lora_table t, oxs_lora_batch b, Place* places) {
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t row = blockIdx.x, r0 = (blockIdx.y * kWaves + wave) * PER;
@@ -175,17 +203,18 @@ __global__ __launch_bounds__(kThreads) void shrink_kernel(oxs_lora_table t, oxs_
     place_row(b, row, a, rank_of(t, a), places);
     return;
   }
-  constexpr uint32_t kAhead = XT == OXS_DTYPE_F32 ? 4 : 8, kStride = 512;
+  constexpr uint32_t kAhead = PER == 1 ? 4 : WT == OXS_DTYPE_F32 ? 1 : 2, kStride = 512;
   const Element<XT>* x = (const Element<XT>*)b.x + (size_t)row * (size_t)b.x_ld;
-  const uint32_t from = lane * 8u;
-  Eight<XT> first[kAhead];
-  if (vec) {
+  const uint32_t eights = t.k & ~7u, from = lane * 8u;
+  const auto at = [&](uint32_t i) { return i < eights ? i : 0u; };
+  Eight<XT> xv[kAhead];
+  if (eights) {
 #pragma unroll
-    for (uint32_t j = 0; j < kAhead; ++j) {
-      first[j] = Eight<XT>{};
-      if (from + j * kStride + 8u <= t.k) first[j] = load_eight<XT>(x + from + j * kStride);
-    }
+    for (uint32_t j = 0; j < kAhead; ++j) xv[j] = load_unaligned<XT>(x + at(from + j * kStride));
   }
+  // the values past the last eight, one in a lane
+  const uint32_t over = eights + lane;
+  const float x_over = lane < 8u && over < t.k ? widen<XT>(x[over]) : 0.0f;
   const uint32_t rank = rank_of(t, a), all_blocks = rank_blocks(t.max_rank);
   // With a rank per wavefront the weights are not waited for until the adapter's rank is known: a slot has room for
   // max_rank whatever it holds.
@@ -196,44 +225,39 @@ __global__ __launch_bounds__(kThreads) void shrink_kernel(oxs_lora_table t, oxs_
   float s[PER];
 #pragma unroll
   for (int p = 0; p < PER; ++p) s[p] = 0.0f;
-  uint32_t i = from;
-  const auto add = [&](const float (&xv)[8]) {
+  for (uint32_t i0 = 0; i0 < eights;) {
+    Eight<WT> wv[kAhead][PER];
 #pragma unroll
-    for (int p = 0; p < PER; ++p) {
-      const Eight<WT> e = load_eight<WT>(w + (size_t)p * kp + i);
+    for (uint32_t j = 0; j < kAhead; ++j)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[p] = __builtin_fmaf(e[j], xv[j], s[p]);
+      for (int p = 0; p < PER; ++p) wv[j][p] = load_eight<WT>(w + (size_t)p * kp + at(i0 + from + j * kStride));
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; ++j) {
+      const bool in = i0 + from + j * kStride < eights;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = in ? xv[j][e] : 0.0f;
+#pragma unroll
+        for (int p = 0; p < PER; ++p) s[p] = __builtin_fmaf(wv[j][p][e], v, s[p]);
+      }
     }
-  };
-  const auto add_eight = [&](const Eight<XT>& e) {
-    float xv[8];
+    i0 += kAhead * kStride;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) xv[j] = e[j];
-    add(xv);
-  };
-  if (vec) {
-#pragma unroll
-    for (uint32_t j = 0; j < kAhead; ++j, i += kStride) {
-      if (i + 8u > t.k) break;
-      add_eight(first[j]);
-    }
-#pragma unroll 4
-    for (; i + 8u <= t.k; i += kStride) add_eight(load_eight<XT>(x + i));
+    for (uint32_t j = 0; j < kAhead; ++j) xv[j] = load_unaligned<XT>(x + at(i0 + from + j * kStride));
   }
-  for (; i < t.k; i += kStride) {
-    float xv[8];
+  if (eights < t.k && lane < 8u) {  // (the table's rows are padded to whole eights)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) xv[j] = i + j < t.k ? widen<XT>(x[i + j]) : 0.0f;
-    add(xv);
+    for (int p = 0; p < PER; ++p) s[p] = __builtin_fmaf(widen<WT>(w[(size_t)p * kp + over]), x_over, s[p]);
   }
+  float v = 0.0f;  // lane p: rank r0 + p's
 #pragma unroll
   for (int p = 0; p < PER; ++p) {
-    float v = s[p];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    // ranks past the adapter's, up to the block's end, are zero
-    if (lane == 0 && r0 + p < rank_blocks(rank) * kBlock) store_value(b.workspace, row, all_blocks, r0 + p, r0 + p < rank ? v * scale : 0.0f);
+    const float sum = wave_sum(s[p]);
+    if (lane == (uint32_t)p) v = sum;
   }
+  // ranks past the adapter's, up to the block's end, are zero
+  if (lane < PER && r0 + lane < rank_blocks(rank) * kBlock)
+    store_value(b.workspace, row, all_blocks, r0 + lane, r0 + lane < rank ? v * scale : 0.0f);
 }
 
 // ---------------------------------------------------------------- y_b += B_a v_b
@@ -297,7 +321,7 @@ struct Cursor {
 // for all of the rows and taken for its own.
 // The operands of the next PF (adapter, rank block) pairs are on their way while one is worked on.
 template <int WT, int YT, int TT, int PF, int RR>
-__global__ __launch_bounds__(kThreads, RR == 4 ? 3 : 2) void expand_kernel(oxs_lora_table t, oxs_lora_batch b, const Place* places,
+__global__ __launch_bounds__(kThreads, RR == 4 || PF == 1 ? 3 : 2) void expand_kernel(oxs_lora_table t, oxs_lora_batch b, const Place* places,
                                                              uint32_t rows, uint32_t col_groups, uint32_t vec) {
   const uint32_t lane = threadIdx.x & 63u, n = lane & 31u, g = lane >> 5;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -318,9 +342,6 @@ __global__ __launch_bounds__(kThreads, RR == 4 ? 3 : 2) void expand_kernel(oxs_l
   const uint16_t* vb = (const uint16_t*)b.workspace + (size_t)my.row * all_blocks * (kValueBytes / 2) + g * 8u;
 
   Cursor ahead;
-  ahead.rest = live;
-  ahead.slot = ahead.rank = 0;
-  ahead.adapter(my.slot, my.rank);
   Eight<WT> w[PF][TT];
   Eight<OXS_DTYPE_BF16> v[PF][kPlanes];
   uint32_t same[PF];
@@ -338,8 +359,15 @@ __global__ __launch_bounds__(kThreads, RR == 4 ? 3 : 2) void expand_kernel(oxs_l
     same[i] = ahead.same;
     ahead.next(my.slot, my.rank);
   };
+  const auto begin = [&]() {
+    ahead.rest = live;
+    ahead.slot = ahead.rank = 0;
+    ahead.adapter(my.slot, my.rank);
 #pragma unroll
-  for (int i = 0; i < PF; ++i) fetch(i);
+    for (int i = 0; i < PF; ++i) fetch(i);
+  };
+  begin();
+  const bool one = same[0] == live;  // adapter for all rows
 
   // y, where a row has an adapter
   const uint32_t mine = live >> (4u * g);  // bit 8 (r / 4) + r % 4: register r's row
@@ -353,61 +381,93 @@ __global__ __launch_bounds__(kThreads, RR == 4 ? 3 : 2) void expand_kernel(oxs_l
   };
   const bool whole = vec != 0u && (uint64_t)(col + 1u) * 32u * TT <= t.m;
   Vec old[RR];
-  if (whole) {
+  const auto load_old = [&]() {
+    if (whole) {
 #pragma unroll
-    for (int r = 0; r < RR; ++r) {
-      const YE* p = y_at(r);
-      if ((mine >> (8 * (r / 4) + r % 4)) & 1u) old[r] = *(const Vec*)p;
+      for (int r = 0; r < RR; ++r) {
+        const YE* p = y_at(r);
+        if ((mine >> (8 * (r / 4) + r % 4)) & 1u) old[r] = *(const Vec*)p;
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < RR; ++r) {
+        const YE* p = y_at(r);
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt)
+          if (((mine >> (8 * (r / 4) + r % 4)) & 1u) && out0 + tt < t.m) old[r].e[tt] = p[tt];
+      }
     }
-  } else {
-#pragma unroll
-    for (int r = 0; r < RR; ++r) {
-      const YE* p = y_at(r);
-#pragma unroll
-      for (int tt = 0; tt < TT; ++tt)
-        if (((mine >> (8 * (r / 4) + r % 4)) & 1u) && out0 + tt < t.m) old[r].e[tt] = p[tt];
-    }
-  }
+  };
+  load_old();
 
-  float acc[TT][RR];
+  typedef float Acc __attribute__((ext_vector_type(RR)));
+  Acc acc[TT];
+  // The products of all adapters. TAKE: computed for all rows and taken for the adapter's own; otherwise onto the sums,
+  // with values of 0 for the other rows.
+  const auto products = [&](auto take) {
+    constexpr bool TAKE = decltype(take)::value;
 #pragma unroll
-  for (int tt = 0; tt < TT; ++tt)
+    for (int tt = 0; tt < TT; ++tt) acc[tt] = Acc{};
+    do {
 #pragma unroll
-    for (int r = 0; r < RR; ++r) acc[tt][r] = 0.0f;
-  do {
+      for (int i = 0; i < PF; ++i) {
+        const uint32_t s = same[i];
+        if (s) {
+          bf16x8 vp[kPlanes];
 #pragma unroll
-    for (int i = 0; i < PF; ++i) {
-      const uint32_t s = same[i];
-      if (s) {
-        bf16x8 vp[kPlanes];
+          for (int q = 0; q < (int)kPlanes; ++q) {
+            u32x4 x = v[i][q].q[0];
+            if constexpr (!TAKE) {
 #pragma unroll
-        for (int q = 0; q < (int)kPlanes; ++q) vp[q] = __builtin_bit_cast(bf16x8, v[i][q].q[0]);
-        const uint32_t bits = s >> (4u * g);
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-          const Parts<WT> wp(w[i][tt]);
-          f32x16 d = {};
-          if (RR == 16 && s == live) {  // one adapter for all: onto the sum
-#pragma unroll
-            for (int r = 0; r < RR; ++r) d[r] = acc[tt][r];
+              for (int j = 0; j < 4; ++j) x[j] = (s >> n) & 1u ? x[j] : 0u;
+            }
+            vp[q] = __builtin_bit_cast(bf16x8, x);
           }
+          const uint32_t bits = s >> (4u * g);
 #pragma unroll
-          for (int sum = 2; sum >= 0; --sum)  // the small products first
+          for (int tt = 0; tt < TT; ++tt) {
+            const Parts<WT> wp(w[i][tt]);
+            f32x16 d = {};
+            if constexpr (!TAKE) {
 #pragma unroll
-            for (int q = 0; q < Parts<WT>::N; ++q)
-              if (q <= sum) d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vp[sum - q], wp.p[q], d, 0, 0, 0);
-          if (RR == 16 && s == live) {
+              for (int r = 0; r < RR; ++r) d[r] = acc[tt][r];
+            }
 #pragma unroll
-            for (int r = 0; r < RR; ++r) acc[tt][r] = d[r];
-          } else {
+            for (int sum = 2; sum >= 0; --sum)  // the small products first
 #pragma unroll
-            for (int r = 0; r < RR; ++r) acc[tt][r] += (bits >> (8 * (r / 4) + r % 4)) & 1u ? d[r] : 0.0f;
+              for (int q = 0; q < Parts<WT>::N; ++q)
+                if (q <= sum) d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vp[sum - q], wp.p[q], d, 0, 0, 0);
+            if constexpr (TAKE) {
+#pragma unroll
+              for (int r = 0; r < RR; ++r) acc[tt][r] += (bits >> (8 * (r / 4) + r % 4)) & 1u ? d[r] : 0.0f;
+            } else {
+#pragma unroll
+              for (int r = 0; r < RR; ++r) acc[tt][r] = d[r];
+            }
           }
         }
+        fetch(i);
       }
-      fetch(i);
+    } while (same[0]);
+  };
+  if constexpr (RR == 4) {
+    products(std::true_type{});
+  } else {
+    products(std::false_type{});
+    if (!one) {
+      // 0 times an infinite weight is NaN in the other rows: once more, then, row by row
+      float bad = 0.0f;
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+        for (int r = 0; r < RR; ++r) bad = __builtin_fmaf(acc[tt][r], 0.0f, bad);
+      if (__ballot(bad != bad)) {
+        begin();
+        products(std::true_type{});
+        load_old();  // (as it is: kept through the second pass, it would not fit in registers)
+      }
     }
-  } while (same[0]);
+  }
 
   const auto sum = [&](int r) {
     Vec z;
@@ -529,20 +589,23 @@ extern "C" int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* b
     constexpr int WT = decltype(wt)::value;
     by_values(b.x_dtype, [&](auto xt) {
       constexpr int XT = decltype(xt)::value;
-      const uint32_t vec = even(b.x, b.x_ld, size_of(XT), 16) ? 1u : 0u;
       if ((uint64_t)b.batch * blocks >= 256u)
-        hipLaunchKernelGGL((shrink_kernel<WT, XT, 4>), dim3(b.batch, blocks + 1u), dim3(kThreads), 0, st, t, b, places,
-                           vec);
+        hipLaunchKernelGGL((shrink_kernel<WT, XT, 4>), dim3(b.batch, blocks + 1u), dim3(kThreads), 0, st, t, b, places);
       else
-        hipLaunchKernelGGL((shrink_kernel<WT, XT, 1>), dim3(b.batch, blocks * 4u + 1u), dim3(kThreads), 0, st, t, b, places,
-                           vec);
+        hipLaunchKernelGGL((shrink_kernel<WT, XT, 1>), dim3(b.batch, blocks * 4u + 1u), dim3(kThreads), 0, st, t, b, places);
     });
     by_values(b.y_dtype, [&](auto yt) {
       constexpr int YT = decltype(yt)::value, TT = WT == OXS_DTYPE_F32 ? 2 : 4;
       const uint32_t vec = even(b.y, b.y_ld, size_of(YT), TT * size_of(YT)) ? 1u : 0u;
-      const uint32_t rows = b.batch <= kFewRows ? 8u : kRows;
-      const uint32_t row_tiles = (b.batch + rows - 1u) / rows;
       uint32_t col_groups = (t.m + 32u * TT * kWaves - 1u) / (32u * TT * kWaves);
+      // Tiles of 8 rows where those of 32 would be too few workgroups for the card: then each waits less, for fewer
+      // adapters. Tiles of 32 and of 8 rows, us, at 126 workgroups (64 rows of 32000 outputs, bf16, rank 16, 64
+      // adapters) 28.6 and 18.3, at 250 (32 rows of 128256, 1 and 32 adapters) 11.4 and 13.7, 31.3 and 30.9, at 500
+      // (64 rows, 1 and 16) 16.5 and 20.1, 24.9 and 25.7; f16 with bf16 outputs and rank 32 at 250 (1 and 32
+      // adapters) 10.0 and 13.2, 85 and 55, at 500 (1 and 16) 14.0 and 21.4, 33.4 and 32.8.
+      const uint32_t few = WT == OXS_DTYPE_F16 ? 256u : 200u;
+      const uint32_t rows = (uint64_t)((b.batch + kRows - 1u) / kRows) * col_groups <= few ? 8u : kRows;
+      const uint32_t row_tiles = (b.batch + rows - 1u) / rows;
       // a multiple of 8: the workgroups of a range of outputs are all on one XCD, whose L2 then holds its weights
       if (row_tiles > 1u) col_groups = (col_groups + 7u) / 8u * 8u;
       const auto go = [&](auto kernel) {
@@ -550,7 +613,7 @@ extern "C" int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* b
                            vec);
       };
       if (rows <= 8u) go(expand_kernel<WT, YT, TT, 2, 4>);
-      else go(expand_kernel<WT, YT, TT, 2, 16>);
+      else go(expand_kernel<WT, YT, TT, YT == OXS_DTYPE_BF16 ? 1 : 2, 16>);
     });
   });
   return launched();

@@ -218,6 +218,43 @@ def test_batches_around_the_kernels_own_sizes(torch_gpu, batch, ranks, w, order)
     check(y, want, bound, f"{batch} {order}")
 
 
+LARGE = [
+    # tiles of 32 rows: batch, m, k, ranks of the slots, weights, x, y, extra elements between y's rows
+    (33, 70001, 24, [16, 3], "f32", "f32", "f32", 0),
+    (65, 40000, 40, [16] * 40, "bf16", "bf16", "f32", 1),
+    (96, 50257, 512, [8, 17], "bf16", "f32", "bf16", 0),
+    (97, 40002, 30, [5, 0, 64], "f32", "f32", "bf16", 2),
+    (150, 36003, 64, [33, 16, 2], "f16", "f32", "f32", 5),
+    (257, 16500, 9, [16] * 20, "f16", "bf16", "bf16", 3),
+    (300, 12001, 77, [256, 1], "bf16", "f32", "f32", 3),
+    (1024, 4100, 20, [12, 16], "bf16", "f32", "f32", 4),
+    (1025, 4099, 16, [4] * 9, "f32", "bf16", "f32", 1),
+    (2100, 2500, 33, [8, 0, 20], "bf16", "f32", "bf16", 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["mixed", "packed"])
+@pytest.mark.parametrize("batch,m,k,ranks,w,xd,yd,pad", LARGE)
+def test_large_tiles_match_the_definition(torch_gpu, batch, m, k, ranks, w, xd, yd, pad, order):
+    t = torch_gpu
+    kinds = {"f32": t.float32, "bf16": t.bfloat16}
+    x, y, ad, dt, g = make(t, batch * 3 + m, batch, m, k, ranks, w)
+    x = x.to(kinds[xd])
+    flat = t.full((batch, m + pad), 7.0, dtype=kinds[yd], device="cuda")
+    yv = flat[:, :m]
+    yv.copy_(y)
+    ids = t.randint(-1, len(ranks) + 1, (batch,), generator=g, device="cuda", dtype=t.int32)
+    if order == "packed":
+        ids = ids.sort().values
+    want, bound = reference(yv, x, ids, ad, yd == "bf16")
+    before = flat.clone()
+    table(t, m, k, ranks, ad, dt, batch).add(yv, x, ids)
+    check(yv, want, bound, f"{batch} x {m}")
+    idle = t.tensor([int(i) not in ad for i in ids.tolist()], device="cuda")
+    assert t.equal(flat[idle], before[idle]) and t.equal(flat[:, m:], before[:, m:])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,k", [(50257, 895), (129, 4095), (6, 513)])
 @pytest.mark.parametrize("w", ["f32", "bf16", "f16"])
@@ -280,6 +317,29 @@ def test_infinities_and_nan_stay_with_their_rows(torch_gpu, batch, dtype):
     check(y[fine], want[fine], bound[fine])
     assert bool(y[5].isnan().all()) and not bool(y[0].isfinite().any())
     assert not bool(y[ids == 1].isfinite().any())  # an infinite value of v meets weights of every output
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,yd", [("f32", "f32"), ("bf16", "f32"), ("f16", "bf16")])
+def test_a_bad_adapter_beside_others_in_large_tiles(torch_gpu, dtype, yd):
+    # enough rows and outputs for tiles of 32 rows, each of several adapters; y of odd and of even strides
+    t = torch_gpu
+    batch, k, ranks = 200, 72, [16, 20, 3, 0, 9]
+    for m in (20001, 26000):
+        x, y, ad, dt, g = make(t, m, batch, m, k, ranks, dtype)
+        y = y.to(t.float32 if yd == "f32" else t.bfloat16)
+        ids = t.randint(-1, 5, (batch,), generator=g, device="cuda", dtype=t.int32)
+        want, bound = reference(y, x, ids, ad, yd == "bf16")
+        bad = ad | {1: (ad[1][0], ad[1][1].clone(), ad[1][2])}
+        bad[1][1][::3, 17] = float("inf")
+        bad[1][1][1::3, 0] = float("nan")
+        before = y.clone()
+        table(t, m, k, ranks, bad, dt, batch).add(y, x, ids)
+        fine = ids != 1
+        check(y[fine], want[fine], bound[fine], f"m={m}")
+        assert not bool(y[~fine][:, ::3].isfinite().any()) and bool(y[~fine][:, 1::3].isnan().all())
+        check(y[~fine][:, 2::3], want[~fine][:, 2::3], bound[~fine][:, 2::3], f"m={m}, outputs of finite weights")
+        assert t.equal(y[(ids < 0) | (ids == 3)], before[(ids < 0) | (ids == 3)])
 
 
 @pytest.mark.gpu
