@@ -763,11 +763,16 @@ __global__ __launch_bounds__(64) void merge_kernel(Params p) {
 template <int DT, bool CAP>
 static void launch(Params& p, hipStream_t st) {
   const oxs_logprobs& b = p.b;
-  // Tiles of 8192 logits (32 per thread), or of 2048 where those would leave CUs without a workgroup.
+  // Tiles of 8192 logits (32 per thread), or of 2048 where those would leave CUs without a workgroup and the join does
+  // not have more to do for it than the rows less. 8192 and 2048, float32, us: no alternatives, 1 row of 32000 7.5 and
+  // 5.4, 24 rows of 50257 8.5 and 6.9, 15 of 128256 8.0 and 7.7; 5 alternatives 1 row of 32000 10.5 and 9.0, 24 rows
+  // 12.0 and 10.7, 60 rows 11.9 and 12.6; 1 row of 128256 with 10 10.7 and 10.2, with 20 11.7 and 12.6.
   const auto tiles_of = [&](uint32_t tile) { return (b.vocab + 7u + tile - 1u) / tile; };
-  const uint32_t large = tiles_of(kThreads * 32);
-  const bool small = (uint64_t)b.rows * large < 256u;
-  const uint32_t tiles = small ? tiles_of(kThreads * 8) : large;
+  const uint32_t large = tiles_of(kThreads * 32), fine = tiles_of(kThreads * 8);
+  const uint64_t groups = (uint64_t)b.rows * large;
+  const bool small =
+      b.top_n ? groups < 150u && fine <= kMaxSplits && fine * b.top_n <= kMergeKeys : groups < 256u;
+  const uint32_t tiles = small ? fine : large;
   // A row is split where its parts fill CUs that whole rows leave idle, by more than the join costs: up to
   // more rows the longer they are. Split and whole, float32, 8 alternatives, us: 4000 logits 110 rows 10.1 and
   // 8.8; 32000 logits 60 rows 12.7 and 19.7, 250 rows 19.1 and 17.9; 128256 logits 250 rows 34.8 and 39.2,
@@ -797,6 +802,7 @@ static void launch(Params& p, hipStream_t st) {
   if (p.splits == 1u) return;
   const auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(b.rows), dim3(64), 0, st, p); };
   if (b.top_n == 0u) join(merge_kernel<DT, CAP, false, 1>);
+  // (ten keys per lane where five would do cost 0.3 us)
   else if (p.splits * b.top_n <= 5u * 64u) join(merge_kernel<DT, CAP, true, 5>);
   else join(merge_kernel<DT, CAP, true, 10>);
 }

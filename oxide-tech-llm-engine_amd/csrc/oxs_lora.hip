@@ -321,7 +321,7 @@ struct Cursor {
 // for all of the rows and taken for its own.
 // The operands of the next PF (adapter, rank block) pairs are on their way while one is worked on.
 template <int WT, int YT, int TT, int PF, int RR>
-__global__ __launch_bounds__(kThreads, RR == 4 || PF == 1 ? 3 : 2) void expand_kernel(oxs_lora_table t, oxs_lora_batch b, const Place* places,
+__global__ __launch_bounds__(kThreads, RR == 4 || (PF == 1 && WT != OXS_DTYPE_F32) ? 3 : 2) void expand_kernel(oxs_lora_table t, oxs_lora_batch b, const Place* places,
                                                              uint32_t rows, uint32_t col_groups, uint32_t vec) {
   const uint32_t lane = threadIdx.x & 63u, n = lane & 31u, g = lane >> 5;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -589,31 +589,40 @@ extern "C" int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* b
     constexpr int WT = decltype(wt)::value;
     by_values(b.x_dtype, [&](auto xt) {
       constexpr int XT = decltype(xt)::value;
-      if ((uint64_t)b.batch * blocks >= 256u)
+      // A wavefront per 4 ranks reads x a quarter as often, one per rank has less to wait for: 128 rows of 4096 inputs,
+      // rank 16, 8.7 and 8.5 us (both products, 2000 outputs), 192 rows 9.0 and 9.7, 1024 rows of rank 32 29 and 44.
+      if ((uint64_t)b.batch * blocks >= 160u)
         hipLaunchKernelGGL((shrink_kernel<WT, XT, 4>), dim3(b.batch, blocks + 1u), dim3(kThreads), 0, st, t, b, places);
       else
         hipLaunchKernelGGL((shrink_kernel<WT, XT, 1>), dim3(b.batch, blocks * 4u + 1u), dim3(kThreads), 0, st, t, b, places);
     });
     by_values(b.y_dtype, [&](auto yt) {
-      constexpr int YT = decltype(yt)::value, TT = WT == OXS_DTYPE_F32 ? 2 : 4;
-      const uint32_t vec = even(b.y, b.y_ld, size_of(YT), TT * size_of(YT)) ? 1u : 0u;
-      uint32_t col_groups = (t.m + 32u * TT * kWaves - 1u) / (32u * TT * kWaves);
-      // Tiles of 8 rows where those of 32 would be too few workgroups for the card: then each waits less, for fewer
-      // adapters. Tiles of 32 and of 8 rows, us, at 126 workgroups (64 rows of 32000 outputs, bf16, rank 16, 64
-      // adapters) 28.6 and 18.3, at 250 (32 rows of 128256, 1 and 32 adapters) 11.4 and 13.7, 31.3 and 30.9, at 500
-      // (64 rows, 1 and 16) 16.5 and 20.1, 24.9 and 25.7; f16 with bf16 outputs and rank 32 at 250 (1 and 32
-      // adapters) 10.0 and 13.2, 85 and 55, at 500 (1 and 16) 14.0 and 21.4, 33.4 and 32.8.
-      const uint32_t few = WT == OXS_DTYPE_F16 ? 256u : 200u;
-      const uint32_t rows = (uint64_t)((b.batch + kRows - 1u) / kRows) * col_groups <= few ? 8u : kRows;
-      const uint32_t row_tiles = (b.batch + rows - 1u) / rows;
-      // a multiple of 8: the workgroups of a range of outputs are all on one XCD, whose L2 then holds its weights
-      if (row_tiles > 1u) col_groups = (col_groups + 7u) / 8u * 8u;
-      const auto go = [&](auto kernel) {
+      constexpr int YT = decltype(yt)::value;
+      const auto groups = [&](uint32_t outputs) { return (t.m + outputs * kWaves - 1u) / (outputs * kWaves); };
+      const auto go = [&](auto kernel, auto width, uint32_t rows) {
+        constexpr uint32_t TT = decltype(width)::value;
+        const uint32_t vec = even(b.y, b.y_ld, size_of(YT), TT * size_of(YT)) ? 1u : 0u;
+        const uint32_t row_tiles = (b.batch + rows - 1u) / rows;
+        uint32_t col_groups = groups(32u * TT);
+        // a multiple of 8: the workgroups of a range of outputs are all on one XCD, whose L2 then holds its weights
+        if (row_tiles > 1u) col_groups = (col_groups + 7u) / 8u * 8u;
         hipLaunchKernelGGL(kernel, dim3(row_tiles * col_groups), dim3(kThreads), 0, st, t, b, places, rows, col_groups,
                            vec);
       };
-      if (rows <= 8u) go(expand_kernel<WT, YT, TT, 2, 4>);
-      else go(expand_kernel<WT, YT, TT, YT == OXS_DTYPE_BF16 ? 1 : 2, 16>);
+      // Tiles of 8 rows where those of 32 would be too few workgroups for the card: then each waits less, for fewer
+      // adapters. Tiles of 32 and of 8 rows, us, rank 16 in bf16: 126 workgroups (64 rows of 32000 outputs, 64
+      // adapters) 28.6 and 18.3; 198 (48 rows of 50257, 1 and 32) 15.9 and 15.3, 34.9 and 28.0; 251 (32 rows of 128256,
+      // 1 and 32) 11.7 and 14.1, 31.4 and 31.0; 502 (64 rows, 1 and 16) 16.6 and 20.1, 25.5 and 26.0. f16, rank 32,
+      // bf16 outputs: 251 (1 and 32) 10.2 and 13.3, 86 and 53; 502 (1 and 16) 13.7 and 21.3, 33.8 and 32.6.
+      const uint32_t few = WT == OXS_DTYPE_F16 ? 256u : 200u;
+      // Outputs per lane in tiles of 8 rows: f32 weights fill the registers at 4 (24 rows of 50257 outputs with an
+      // adapter each: 18.5 us with 2, 22.0 with 4), the others' loads are wider for it (64 rows of 32000, 8 adapters:
+      // 11.9 with 2, 9.5 with 4).
+      constexpr int kFew = WT == OXS_DTYPE_F32 ? 2 : 4;
+      if ((uint64_t)((b.batch + kRows - 1u) / kRows) * groups(128u) <= few)
+        go(expand_kernel<WT, YT, kFew, 2, 4>, Int<kFew>{}, 8u);
+      else
+        go(expand_kernel<WT, YT, 4, YT == OXS_DTYPE_BF16 ? 1 : 2, 16>, Int<4>{}, kRows);
     });
   });
   return launched();
