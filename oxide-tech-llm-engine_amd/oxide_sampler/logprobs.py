@@ -117,7 +117,7 @@ class TokenLogprobs:
 
     def launch(self, call: OxsLogprobs, stream=None) -> None:
         """Launches a described call on `stream` (torch stream or None)."""
-        s = stream if stream is not None else self.torch.cuda.current_stream(self.device)
+        s = stream if stream is not None else self.torch.cuda.current_stream(self.device.index)
         if self.torch.cuda.current_device() != self.device.index:
             with self.torch.cuda.device(self.device):
                 check(self.lib.oxs_token_logprobs(call, s.cuda_stream), "oxs_token_logprobs")

@@ -62,7 +62,7 @@ class LoraAdapters:
         self.table.ranks, self.table.scales = self.ranks.data_ptr(), self.scales.data_ptr()
 
     def _call(self, name, stream, *args):
-        s = stream if stream is not None else self.torch.cuda.current_stream(self.device)
+        s = stream if stream is not None else self.torch.cuda.current_stream(self.device.index)
         call = getattr(self.lib, name)
         if self.torch.cuda.current_device() != self.device.index:
             with self.torch.cuda.device(self.device):
