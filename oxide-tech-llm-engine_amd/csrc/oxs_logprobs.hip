@@ -31,7 +31,7 @@ constexpr float kLn2 = 0.693147180559945309417f;
 // 2^-256 is 0 in 32 bits: a difference below this (or NaN, of two infinities) adds nothing
 constexpr float kFloor = -256.0f;
 constexpr uint32_t kMaxSplits = 64;      // parts of a row
-constexpr uint32_t kMaxParts = 4096;     // rows * parts of a call that splits its rows
+constexpr uint32_t kMaxParts = 4096;     // rows * (parts + 1) of a call that splits its rows, at most
 constexpr uint32_t kMergeKeys = 10 * 64; // parts * top_n of a split row
 constexpr uint32_t kRoom = OXS_LOGPROBS_MAX_TOP + 512;  // candidates of a wavefront: those kept, and 64 lanes' next 8
 
@@ -42,7 +42,8 @@ struct Params {
   // a split row's parts, in the workspace: [row * splits + part]
   float4* stats;    // m (raw logit), s, t
   uint64_t* keys;   // [top_n] the part's largest keys, in order, 0 past the last
-  uint32_t* counts; // [tokens_per_row] tokens of the part in front of each given token
+  // [row][splits + 1][tokens_per_row]: tokens of each part in front of the given tokens, then the tokens' logits
+  uint32_t* counts;
 };
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
@@ -219,6 +220,18 @@ __device__ __forceinline__ uint32_t keep_largest(uint64_t* keys, uint32_t count,
   return kept;
 }
 
+// How many of the `all` keys of a list in LDS, with kAhead - 1 zeros or more behind them, are above a key. Eight at a
+// time, so that their reads overlap.
+constexpr uint32_t kAhead = 8;
+__device__ __forceinline__ uint32_t keys_above(const uint64_t* list, uint32_t all, uint64_t key) {
+  uint32_t n = 0;
+  for (uint32_t i = 0; i < all; i += kAhead) {
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; ++j) n += list[i + j] > key ? 1u : 0u;
+  }
+  return n;
+}
+
 // ---------------------------------------------------------------- the pass over the logits
 
 // The parameters as they lie in memory, for what is needed after the pass only: read where they are used, they take
@@ -334,7 +347,7 @@ __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
   __shared__ __align__(16) float s_stage[TOP ? kWaves : 1][TOP ? 512 : 4];
   __shared__ uint32_t s_stage_id[TOP ? kWaves : 1][TOP ? kStage : 1];
   __shared__ uint32_t s_order[2][TOP ? kThreads : 1];
-  __shared__ uint64_t s_list[TOP ? kThreads : 1];
+  __shared__ __align__(16) uint64_t s_list[TOP ? kThreads + kAhead : 1];
   __shared__ float s_m[kWaves], s_s[kWaves], s_t[kWaves];
   __shared__ uint32_t s_count[kWaves];
   __shared__ uint32_t s_before[kWaves][OXS_LOGPROBS_MAX_TOKENS];
@@ -649,6 +662,7 @@ __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
       all += s_count[w];
     }
     if (lane < count) s_list[before_me + lane] = keys[lane];
+    if (tid < kAhead) s_list[all + tid] = 0;
     __syncthreads();
   }
   before = 0;  // tokens of this part in front of given token tid
@@ -660,13 +674,14 @@ __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
   uint32_t place = kNoToken;
   if (TOP && tid < all) {
     mine = s_list[tid];
-    place = 0;
-    for (uint32_t i = 0; i < all; ++i) place += s_list[i] > mine ? 1u : 0u;
+    place = keys_above(s_list, all, mine);
   }
   if (late.splits > 1u) {
     const size_t at = (size_t)row * late.splits + part;
     if (tid == 0) late.stats[at] = make_float4(bm, bs, bt, 0.0f);
-    if (tid < T) late.counts[at * T + tid] = before;
+    uint32_t* counts = late.counts + (size_t)row * (late.splits + 1u) * T;
+    if (tid < T) counts[part * T + tid] = before;
+    if (tid < T && part == 0u) counts[late.splits * T + tid] = __float_as_uint(want_l);
     if (TOP && place < N) late.keys[at * N + place] = mine;
     if (TOP && tid >= all && tid < N) late.keys[at * N + tid] = 0;
     return;
@@ -679,27 +694,36 @@ __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
 }
 
 // One wavefront joins the parts of a row. The alternatives are the keys no less than a bound that is found by halving
-// a range of keys until N to N + 4 of them are above it.
-template <int DT, bool CAP, bool TOP, int PER>
+// a range of keys until N to N + 4 of them are above it. All that it reads is on its way before the first is waited for
+// (the counts of the ninth token on aside).
+template <bool CAP, bool TOP, int PER>
 __global__ __launch_bounds__(64) void merge_kernel(Params p) {
   const oxs_logprobs& b = p.b;
   const uint32_t row = blockIdx.x, lane = threadIdx.x;
   const uint32_t S = p.splits, T = b.tokens_per_row, N = TOP ? b.top_n : 0u;
-  __shared__ uint64_t s_best[64];
+  __shared__ __align__(16) uint64_t s_best[64 + kAhead];
   const size_t at = (size_t)row * S;
-  float4 st = make_float4(neg_inf(), 0.0f, 0.0f, 0.0f);
-  if (lane < S) st = p.stats[at + lane];
+  const uint32_t part = min(lane, S - 1u);
+  float4 st = p.stats[at + part];
   uint64_t k[PER], floor = ~0ull;
   if constexpr (TOP) {
+    const uint32_t last = S * N - 1u;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) k[i] = lane + 64u * i < S * N ? p.keys[at * N + lane + 64u * i] : 0;
+    for (int i = 0; i < PER; ++i) k[i] = p.keys[at * N + min(lane + 64u * i, last)];
     // the ceil(N / S)-th key of each part: N keys at least are no less than the smallest of them
-    if (lane < S) floor = p.keys[(at + lane) * N + (N + S - 1u) / S - 1u];
+    floor = p.keys[(at + part) * N + (N + S - 1u) / S - 1u];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) k[i] = lane + 64u * i <= last ? k[i] : 0;
   }
-  uint32_t want = kNoToken;
-  if (lane < T) want = b.tokens[(size_t)row * (size_t)b.tokens_ld + lane];
-  const float want_l = present_logit<DT>(b, row, want);
-  const float inv = inverse_temperature(b, row), c = inv * kLog2e, cap = b.logit_softcap, inv_cap = CAP ? inverse_cap(cap) : 0.0f;
+  const uint32_t* counts = p.counts + (size_t)row * (S + 1u) * T;
+  const auto count_of = [&](uint32_t j) { return counts[part * T + min(j, max(T, 1u) - 1u)]; };
+  uint32_t some[kAhead];
+#pragma unroll
+  for (uint32_t j = 0; j < kAhead; ++j) some[j] = count_of(j);
+  const float want_l = __uint_as_float(counts[S * T + min(lane, max(T, 1u) - 1u)]);
+  if (lane >= S) st = make_float4(neg_inf(), 0.0f, 0.0f, 0.0f);
+  const float inv = inverse_temperature(b, row), c = inv * kLog2e, cap = b.logit_softcap,
+              inv_cap = CAP ? inverse_cap(cap) : 0.0f;
   const auto y_of = [&](float l) {
     if constexpr (CAP) return l == neg_inf() ? l : softcap_of(l, cap, inv_cap);
     else return l;
@@ -709,9 +733,16 @@ __global__ __launch_bounds__(64) void merge_kernel(Params p) {
   const Row r(b, inv, m, wave_sum(f * st.y), wave_sum(f * __builtin_fmaf(d, st.y, st.z)));
   if (lane == 0) r.write(b, row);
   uint32_t before = 0;
-  for (uint32_t j = 0; j < T; ++j) {
-    const uint32_t n = wave_sum(lane < S ? p.counts[(at + lane) * T + j] : 0u);
-    if (lane == j) before = n;
+  for (uint32_t j0 = 0; j0 < T; j0 += kAhead) {
+    if (j0) {
+#pragma unroll
+      for (uint32_t j = 0; j < kAhead; ++j) some[j] = count_of(j0 + j);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; ++j) {
+      const uint32_t n = wave_sum(lane < S ? some[j] : 0u);
+      if (lane == j0 + j) before = n;
+    }
   }
   if (lane < T) r.write_token(b, row, lane, want_l, before);
   if constexpr (TOP) {
@@ -727,12 +758,12 @@ __global__ __launch_bounds__(64) void merge_kernel(Params p) {
     for (int i = 0; i < PER; ++i) n += (uint32_t)__popcll(__ballot(k[i] >= lo));
     for (int step = 0; step < 64 && n > N + 4u; ++step) {
       const uint64_t mid = lo + (hi - lo) / 2u;
-      uint32_t some = 0;
+      uint32_t above = 0;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) some += (uint32_t)__popcll(__ballot(k[i] >= mid));
-      if (some >= N) {
+      for (int i = 0; i < PER; ++i) above += (uint32_t)__popcll(__ballot(k[i] >= mid));
+      if (above >= N) {
         lo = mid;
-        n = some;
+        n = above;
       } else {
         hi = mid;
       }
@@ -747,13 +778,13 @@ __global__ __launch_bounds__(64) void merge_kernel(Params p) {
       all += (uint32_t)__popcll(who);
     }
     all = min(all, 64u);
+    if (lane < kAhead) s_best[all + lane] = 0;
     wave_sync();
     uint32_t place = kNoToken;
     uint64_t mine = 0;
     if (lane < all) {
       mine = s_best[lane];
-      place = 0;
-      for (uint32_t i = 0; i < all; ++i) place += s_best[i] > mine ? 1u : 0u;
+      place = keys_above(s_best, all, mine);
     }
     if (place < N) r.write_top(b, row, place, mine);
     if (lane >= all && lane < N) r.write_top(b, row, lane, 0);
@@ -801,10 +832,10 @@ static void launch(Params& p, hipStream_t st) {
   else by_mask(std::integral_constant<int, 32>{});
   if (p.splits == 1u) return;
   const auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(b.rows), dim3(64), 0, st, p); };
-  if (b.top_n == 0u) join(merge_kernel<DT, CAP, false, 1>);
+  if (b.top_n == 0u) join(merge_kernel<CAP, false, 1>);
   // (ten keys per lane where five would do cost 0.3 us)
-  else if (p.splits * b.top_n <= 5u * 64u) join(merge_kernel<DT, CAP, true, 5>);
-  else join(merge_kernel<DT, CAP, true, 10>);
+  else if (p.splits * b.top_n <= 5u * 64u) join(merge_kernel<CAP, true, 5>);
+  else join(merge_kernel<CAP, true, 10>);
 }
 
 }  // namespace oxs_lp
