@@ -7,8 +7,24 @@
 // H's two terms are both >= 0, so nothing cancels. Differences to m are taken
 // before the scaling, so large logits lose nothing either.
 //
-// rows_kernel: a workgroup reads a part of a row in tiles that stay in registers; each thread keeps its own m, s and
-// t. merge_kernel: a wavefront joins the parts of a row where it was split over workgroups (few rows).
+// rows_kernel: a workgroup reads a part of a row in tiles that stay in
+// registers, the next tile's loads on their way while one is worked on; each
+// thread keeps its own m, s and t, so the row is read once whatever is asked
+// of it. merge_kernel: a wavefront joins the parts of a row where it was split
+// over workgroups (few rows). Alternatives: the N-th largest of the 256
+// threads' maxima is a bound that at least N logits reach, so only the few
+// threads with a logit above it hold candidates; ranks are counted tile by
+// tile against the given tokens' logits.
+//
+// What bounds it: long rows the read (512 rows of 262144 float32 86.6 us,
+// 6.2 TB/s, where a kernel that only reads takes 77), bf16 the vector unit
+// beside it (an exponential, four more operations and a comparison per logit,
+// twice the logits per byte: 2048 rows of 128256 101 us, 5.2 TB/s), decode
+// batches the start, the selection and the join (64 rows of 128256 float32, 20
+// alternatives: 20.0 us, of which the read alone takes 6.5 and the join 4),
+// one row two launches (32000 logits 9.6 us, 8.6 from a graph). A join in the
+// same launch, by the last workgroup of a row to finish, was no faster (16 rows
+// 10.6 us for 4.6 and 2.3; 64 rows equal).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -286,7 +302,9 @@ constexpr float kSlack = 16.0f;
 constexpr float kHuge = 1e31f;  // y c cannot overflow below this, as c <= 10^6 log2 e
 struct Sums {
   float ref = -__builtin_inff(), rc = 0.0f, s = 0.0f, t = 0.0f;
-  __device__ __forceinline__ float rest(float c) const { return fabsf(ref) < kHuge ? __builtin_fmaf(ref, c, -rc) : 0.0f; }
+  __device__ __forceinline__ float rest(float c) const {
+    return fabsf(ref) < kHuge ? __builtin_fmaf(ref, c, -rc) : 0.0f;
+  }
   __device__ __forceinline__ void shift(float by) {  // q + by in the place of q
     const float f = exp2_fast(by);
     t = f * __builtin_fmaf(by, s, t);
@@ -584,7 +602,8 @@ __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
     for (uint32_t j = 0; j < T; ++j) {
       const float l = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(want_l), (int)j));
       if (l == neg_inf()) continue;
-      const float below = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(want_below), (int)j));
+      const float below =
+          __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(want_below), (int)j));
       const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)want, (int)j);
       uint32_t k = 0;
       if (begin + kTile <= (int64_t)id || begin > (int64_t)id) {
@@ -595,7 +614,8 @@ __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
           uint64_t in[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) in[e] = __ballot(v[e0 + e] > than);
-          asm("" : "+s"(in[0]), "+s"(in[1]), "+s"(in[2]), "+s"(in[3]), "+s"(in[4]), "+s"(in[5]), "+s"(in[6]), "+s"(in[7]));
+          asm("" : "+s"(in[0]), "+s"(in[1]), "+s"(in[2]), "+s"(in[3]), "+s"(in[4]), "+s"(in[5]), "+s"(in[6]),
+                   "+s"(in[7]));
 #pragma unroll
           for (int e = 0; e < 8; ++e) k += (uint32_t)__popcll(in[e]);
         }

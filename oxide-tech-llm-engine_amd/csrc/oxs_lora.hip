@@ -1,9 +1,25 @@
 // oxs_lora.hip — low-rank adapters of many requests beside the projection
 // that they share: y_b += B_a (s_a A_a x_b) for the adapter a of each row b.
 //
-// shrink_kernel: v_b = s_a A_a x_b into the workspace. expand_kernel:
-// y_b += B_a v_b on the matrix cores, 32 rows x 64 or 128 outputs per
-// wavefront, for each adapter among the 32 rows in turn.
+// shrink_kernel: v_b = s_a A_a x_b into the workspace, a wavefront per row and
+// one or four ranks. expand_kernel: y_b += B_a v_b on the matrix cores, 32
+// rows (few: 8) in order of adapter x 64 or 128 outputs per wavefront, for each
+// adapter among the rows in turn.
+//
+// What bounds it: large batches the read and write of y (1024 rows of 128256
+// float32 in 8 runs, rank 32: 236 us, 1.13 GB, 4.8 TB/s, a copy's rate; 64 rows,
+// 16 adapters of rank 16: 24.8 us, 4.7 TB/s). f16 weights their conversion and
+// the matrix instructions (256 rows of 151936, 4 adapters of rank 64, bf16 x and
+// y: 67 us for 210 MB; 48 at a copy's rate). Rows with an adapter each the chain
+// of loads (24 rows of 50257, float32 of rank 8: 17.7 us for 42 MB); one row the
+// two launches (32000 outputs, 4096 inputs: 8.9 us, 6.3 from a graph).
+//
+// Left out, measured: the first product on the matrix cores for rows that share
+// an adapter (1024 rows 48 to 90 us, 24 here) or four rows per wavefront (44);
+// row tiles of 64 (prompts 276 us for 230, f16 98 for 76); v through LDS (one row
+// 7.0 us for 5.3); three or four pairs of operands on their way (registers
+// spill: prompts 375 us for 232); row tiles side by side (prompts 259 us for 231)
+// or in chunks of 32 to 256 ranges of outputs (within 5% either way).
 //
 // The matrix cores take bf16. A float is the sum of three bf16 (each the
 // nearest to what is left of it: 2^-9 of it remains after one, 2^-18 after
@@ -159,7 +175,8 @@ __device__ __forceinline__ void place_row(const oxs_lora_batch& b, uint32_t row,
   const uint32_t start = row - row % kWindow, n = min(b.batch - start, kWindow);
   uint32_t other[kWindow / kThreads];  // (all loads before the first is waited for)
 #pragma unroll
-  for (uint32_t i = 0; i < kWindow / kThreads; ++i) other[i] = b.adapters[start + min(threadIdx.x + i * kThreads, n - 1u)];
+  for (uint32_t i = 0; i < kWindow / kThreads; ++i)
+    other[i] = b.adapters[start + min(threadIdx.x + i * kThreads, n - 1u)];
   uint32_t before = 0;
 #pragma unroll
   for (uint32_t i = 0; i < kWindow / kThreads; ++i) {
@@ -191,8 +208,9 @@ __device__ __forceinline__ float wave_sum(float x) {
 
 // One wavefront per (row, PER ranks): its lanes take eight values of x at a time. The loads of kAhead times 512 values
 // are on their way together, those of the first x before the row's adapter is known; lanes past the end load what
-// others do, for nothing: a load behind a branch would be waited for on its own. The last workgroup of a row finds the
-// row's place instead.
+// others do, for nothing: a load behind a branch would be waited for on its own (64 rows of 4096 values, 16 ranks: 6.8
+// us so, 4.7 here). The last workgroup of a row finds the row's place instead. Twice and four times kAhead: 7.7 and
+// 13.8 us for 7.3 (256 rows of 2048, f16 of rank 64), as fewer wavefronts fit.
 template <int WT, int XT, int PER>
 __global__ __launch_bounds__(kThreads) void shrink_kernel(oxs_lora_table t, oxs_lora_batch b, Place* places) {
   const uint32_t lane = threadIdx.x & 63u;
@@ -315,14 +333,17 @@ struct Cursor {
 };
 
 // One wavefront: `rows` <= 32 rows (in order of adapter; at most 8 with RR = 4, where only the first four registers of
-// a tile hold any) x 32 TT outputs (lane n: outputs TT n .. TT n + TT - 1); a
-// workgroup: the same rows and kWaves ranges of outputs side by side. The rows are the first operand, the outputs the
-// second, so a register holds one row's 32 TT outputs side by side over 32 lanes. Each adapter's product is computed
-// for all of the rows and taken for its own.
-// The operands of the next PF (adapter, rank block) pairs are on their way while one is worked on.
+// a tile hold any) x 32 TT outputs (lane n: outputs TT n .. TT n + TT - 1); a workgroup: the same rows and kWaves
+// ranges of outputs side by side. The rows are the first operand, the outputs the second, so a register holds one
+// row's 32 TT outputs side by side over 32 lanes. With RR = 16 every product goes onto the same sums, the values of
+// the rows of other adapters being 0 (128 selections per adapter and rank block less: f16 93 -> 77 us, as above);
+// with RR = 4 it is computed for all of the rows and taken for the adapter's own.
+// The operands of the next PF (adapter, rank block) pairs are on their way while one is worked on. With 16-bit y and
+// weights one leaves registers for a third wavefront per SIMD: 2048 rows of 32000, one adapter, 56 us for 64; with
+// float32 y it does not (256 rows of 128256, 8 adapters of rank 64, 100 us for 95).
 template <int WT, int YT, int TT, int PF, int RR>
-__global__ __launch_bounds__(kThreads, RR == 4 || (PF == 1 && WT != OXS_DTYPE_F32) ? 3 : 2) void expand_kernel(oxs_lora_table t, oxs_lora_batch b, const Place* places,
-                                                             uint32_t rows, uint32_t col_groups, uint32_t vec) {
+__global__ __launch_bounds__(kThreads, RR == 4 || (PF == 1 && WT != OXS_DTYPE_F32) ? 3 : 2) void expand_kernel(
+    oxs_lora_table t, oxs_lora_batch b, const Place* places, uint32_t rows, uint32_t col_groups, uint32_t vec) {
   const uint32_t lane = threadIdx.x & 63u, n = lane & 31u, g = lane >> 5;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t row_tile = blockIdx.x / col_groups;
@@ -474,7 +495,8 @@ __global__ __launch_bounds__(kThreads, RR == 4 || (PF == 1 && WT != OXS_DTYPE_F3
     if constexpr (YT == OXS_DTYPE_BF16 && TT % 2 == 0) {
 #pragma unroll
       for (int tt = 0; tt < TT; tt += 2) {
-        const uint32_t pair = narrow2(widen<YT>(old[r].e[tt]) + acc[tt][r], widen<YT>(old[r].e[tt + 1]) + acc[tt + 1][r]);
+        const uint32_t pair =
+            narrow2(widen<YT>(old[r].e[tt]) + acc[tt][r], widen<YT>(old[r].e[tt + 1]) + acc[tt + 1][r]);
         z.e[tt] = (YE)pair;
         z.e[tt + 1] = (YE)(pair >> 16);
       }
@@ -549,7 +571,8 @@ extern "C" int oxs_lora_load(const oxs_lora_table* table, uint32_t slot, const v
   if (rank) {
     const uint32_t es = size_of(table->dtype);
     if (!a || !b || !aligned(a, es) || !aligned(b, es)) return OXS_ERR_INVALID_ARGUMENT;
-    if ((rank > 1 && a_ld < (int64_t)table->k) || (table->m > 1 && b_ld < (int64_t)rank)) return OXS_ERR_INVALID_ARGUMENT;
+    if ((rank > 1 && a_ld < (int64_t)table->k) || (table->m > 1 && b_ld < (int64_t)rank))
+      return OXS_ERR_INVALID_ARGUMENT;
   }
   by_weights(table->dtype, [&](auto wt) {
     using E = Element<decltype(wt)::value>;
@@ -594,7 +617,8 @@ extern "C" int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* b
       if ((uint64_t)b.batch * blocks >= 160u)
         hipLaunchKernelGGL((shrink_kernel<WT, XT, 4>), dim3(b.batch, blocks + 1u), dim3(kThreads), 0, st, t, b, places);
       else
-        hipLaunchKernelGGL((shrink_kernel<WT, XT, 1>), dim3(b.batch, blocks * 4u + 1u), dim3(kThreads), 0, st, t, b, places);
+        hipLaunchKernelGGL((shrink_kernel<WT, XT, 1>), dim3(b.batch, blocks * 4u + 1u), dim3(kThreads), 0, st, t, b,
+                           places);
     });
     by_values(b.y_dtype, [&](auto yt) {
       constexpr int YT = decltype(yt)::value;
@@ -605,6 +629,7 @@ extern "C" int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* b
         const uint32_t row_tiles = (b.batch + rows - 1u) / rows;
         uint32_t col_groups = groups(32u * TT);
         // a multiple of 8: the workgroups of a range of outputs are all on one XCD, whose L2 then holds its weights
+        // (prompts as above 228 -> 223 us)
         if (row_tiles > 1u) col_groups = (col_groups + 7u) / 8u * 8u;
         hipLaunchKernelGGL(kernel, dim3(row_tiles * col_groups), dim3(kThreads), 0, st, t, b, places, rows, col_groups,
                            vec);

@@ -316,6 +316,24 @@ def test_matches_the_definition(torch_gpu, rows, V, dtype, T, top, mask, temps, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,V,dtype,T,top", [(3, 40000, "f32", 64, 5), (1, 262147, "bf16", 64, 32),
+                                                (200, 70001, "bf16", 9, 0), (141, 90000, "f32", 17, 7),
+                                                (511, 300001, "bf16", 3, 1), (16, 128256, "f32", 8, 10),
+                                                (11, 128256, "f32", 2, 11), (149, 8100, "f32", 33, 3)])
+def test_split_rows_with_many_tokens(torch_gpu, rows, V, dtype, T, top):
+    rng = np.random.default_rng(V + T)
+    x = bf16(wl.zipf_prior_logits(rng, min(rows, 8), V, 3.0))[np.arange(rows) % min(rows, 8)]
+    x[rows // 2, ::2] = NINF
+    t = rng.uniform(0.5, 2.0, rows).astype(np.float32)
+    tokens = some_tokens(x, T, rng)
+    n = min(rows, 8)  # (the rows repeat: the reference of the first and of the changed one is enough)
+    pick = np.unique(np.r_[np.arange(n), rows // 2, rows - 1])
+    got = run(torch_gpu, x, tokens, top, temperatures=t, dtype=dtype)
+    ref = reference(x[pick], tokens[pick], top, temperatures=t[pick])
+    check({k: v[pick] for k, v in got.items()}, ref, V, temperatures=t[pick], what=f"rows={rows} V={V}")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V,dtype", [(5, "f32"), (100, "bf16"), (1500, "f32"), (9000, "bf16"), (33000, "f32")])
 @pytest.mark.parametrize("top", [0, 3, 32])
 def test_special_rows(torch_gpu, V, dtype, top):
