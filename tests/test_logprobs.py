@@ -535,6 +535,46 @@ def test_graphs_streams_and_repeats(torch_gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,V", [(1, 40), (3, 33000), (70, 9000), (520, 2000)])
+def test_memory_behind_the_rows_stays_as_it_was(torch_gpu, rows, V):
+    from oxide_sampler import TokenLogprobs
+    t = torch_gpu
+    x = t.randn(rows, V, device="cuda")
+    tokens = t.randint(0, V, (rows, 3), device="cuda", dtype=t.int32)
+    shapes = {"logsumexp": (), "entropy": (), "status": (), "logprobs": (3,), "ranks": (3,), "top_ids": (4,),
+              "top_logprobs": (4,)}
+    whole = {n: t.full((rows + 2, *s), 77, dtype=t.int32 if n in ("status", "ranks", "top_ids") else t.float32,
+                       device="cuda") for n, s in shapes.items()}
+    lp = TokenLogprobs()
+    lp.compute(x, tokens, top=4, out={n: w[1:rows + 1] for n, w in whole.items()})
+    fresh = lp.compute(x, tokens, top=4)
+    for n, w in whole.items():
+        assert t.equal(w[1:rows + 1], fresh[n]), n
+        assert bool((w[0] == 77).all()) and bool((w[rows + 1:] == 77).all()), n
+
+
+@pytest.mark.gpu
+def test_outputs_on_another_stream(torch_gpu):
+    from oxide_sampler import TokenLogprobs
+    t = torch_gpu
+    x = t.randn(40, 50000, device="cuda")
+    tokens = t.randint(0, 50000, (40,), device="cuda", dtype=t.int32)
+    want = TokenLogprobs().compute(x, tokens, top=6)
+    s = t.cuda.Stream()
+    s.wait_stream(t.cuda.current_stream())
+    lp = TokenLogprobs()
+    outs = []
+    for _ in range(5):
+        junk = [t.zeros(40, device="cuda") for _ in range(3)]  # freed and reused on the current stream
+        outs.append(lp.compute(x, tokens, top=6, stream=s))
+        del junk
+    s.synchronize()
+    for o in outs:
+        for n in want:
+            assert t.equal(o[n], want[n]), n
+
+
+@pytest.mark.gpu
 def test_one_workspace_for_calls_of_all_sizes(torch_gpu):
     # rows split over workgroups in different ways, one call after the other on one workspace
     from oxide_sampler import TokenLogprobs

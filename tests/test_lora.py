@@ -422,6 +422,46 @@ def test_slots_change_in_stream_order_and_under_a_graph(torch_gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch,m", [(1, 700), (5, 700), (9, 3000), (100, 30000), (1025, 5000)])
+def test_rows_behind_the_last_stay_as_they_were(torch_gpu, batch, m):
+    t = torch_gpu
+    x, y, ad, dt, g = make(t, m, batch + 40, m, 48, [16, 7])
+    ids = t.randint(0, 2, (batch + 40,), generator=g, device="cuda", dtype=t.int32)
+    want, bound = reference(y[:batch], x[:batch], ids[:batch], ad)
+    behind = y[batch:].clone()
+    lora = table(t, m, 48, [16, 7], ad, dt, batch + 40)
+    lora.add(y[:batch], x[:batch], ids[:batch])
+    check(y[:batch], want, bound)
+    assert t.equal(y[batch:], behind)
+
+
+@pytest.mark.gpu
+def test_two_calls_on_one_table_at_once(torch_gpu):
+    # the table is read only: a workspace each is all that two streams need
+    t = torch_gpu
+    m, k, batch, ranks = 20000, 512, 100, [16, 8, 30]
+    x, y, ad, dt, g = make(t, 31, batch, m, k, ranks)
+    lora = table(t, m, k, ranks, ad, dt, batch)
+    ids = t.randint(0, 3, (batch,), generator=g, device="cuda", dtype=t.int32)
+    want = lora.add(y.clone(), x, ids)
+    second = t.empty_like(lora.workspace)
+    streams = [t.cuda.Stream(), t.cuda.Stream()]
+    ys = [[y.clone() for _ in range(6)] for _ in streams]
+    calls = [[lora.descriptor(z, x, ids) for z in zs] for zs in ys]
+    for c in calls[1]:
+        c.workspace = second.data_ptr()
+    for s in streams:
+        s.wait_stream(t.cuda.current_stream())
+    for i in range(6):
+        for s, cs in zip(streams, calls):
+            lora.launch(cs[i], s)
+    t.cuda.synchronize()
+    for zs in ys:
+        for z in zs:
+            assert t.equal(z, want)
+
+
+@pytest.mark.gpu
 def test_another_stream_and_repeated_calls(torch_gpu):
     t = torch_gpu
     x, y, ad, dt, g = make(t, 3, 50, 1200, 300, [16, 16])
