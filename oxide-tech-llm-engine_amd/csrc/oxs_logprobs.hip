@@ -604,6 +604,9 @@ __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
       if (l == neg_inf()) continue;
       const float below =
           __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(want_below), (int)j));
+      // None of the wavefront's logits is in front, in most tiles for a likely token (700 rows of 50257, 16 tokens: the
+      // likeliest 92 -> 70 us, drawn ones 91 -> 84, any 90 -> 92).
+      if (!__ballot(top > below)) continue;
       const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)want, (int)j);
       uint32_t k = 0;
       if (begin + kTile <= (int64_t)id || begin > (int64_t)id) {
