@@ -153,6 +153,9 @@ __device__ __forceinline__ float inverse_temperature(const oxs_logprobs& b, uint
   return t > 1e-6f ? 1.0f / t : 1.0f;
 }
 
+// 1 / T to the base 2; above 0 for an infinite T too, so that a difference to -inf stays infinite
+__device__ __forceinline__ float binary_scale(float inv) { return fmaxf(inv * kLog2e, 1.2e-38f); }
+
 // The logit of token i, -inf when it is not present.
 template <int DT>
 __device__ __forceinline__ float present_logit(const oxs_logprobs& b, uint32_t row, uint32_t i) {
@@ -280,13 +283,14 @@ __device__ __forceinline__ float largest_of(const float* v) {
   }
   return __uint_as_float(hi >= 0 ? (uint32_t)hi : lo);
 }
-__device__ __forceinline__ float largest_of_pairs(u32x4 raw) {
-  const uint32_t first = raw[0];
+template <int N>
+__device__ __forceinline__ float largest_of_pairs(const u32x4* raw) {
+  const uint32_t first = raw[0][0];
   i16x2 hi = __builtin_bit_cast(i16x2, first);
   u16x2 lo = __builtin_bit_cast(u16x2, first);
 #pragma unroll
-  for (int i = 1; i < 4; ++i) {
-    const uint32_t x = raw[i];  // (a bit cast of the element itself takes element 0)
+  for (int i = 1; i < 4 * N; ++i) {
+    const uint32_t x = raw[i / 4][i % 4];  // (a bit cast of the element itself takes element 0)
     hi = __builtin_elementwise_max(hi, __builtin_bit_cast(i16x2, x));
     lo = __builtin_elementwise_min(lo, __builtin_bit_cast(u16x2, x));
   }
@@ -319,9 +323,7 @@ struct Sums {
     if (settled) return;
     shift(rest(c));
   }
-  __device__ __forceinline__ bool behind(float top, float c) const {
-    return (top - ref) * c > kSlack || (ref == neg_inf() && top > ref);
-  }
+  __device__ __forceinline__ bool behind(float top, float c) const { return (top - ref) * c > kSlack; }
   __device__ __forceinline__ bool huge() const { return fabsf(ref) >= kHuge && ref > neg_inf(); }
   // N more logits, of which none is 2^kSlack above ref
   template <int N, class Y>
@@ -354,7 +356,6 @@ __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
   constexpr int G = group_size<DT>(), NG = E / G;
   constexpr uint32_t kSize = DT == OXS_DTYPE_F32 ? 4 : 2;
   constexpr uint32_t kTile = kThreads * E;
-  constexpr int kStep = 8;  // logits that are summed while the next are still on their way
   const oxs_logprobs& b = p.b;
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
   const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
@@ -374,7 +375,7 @@ __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
   // logits between the boundary before the row and its first one
   const uint32_t skip = ((uint32_t)(uintptr_t)base & 15u) / kSize;
   const uint32_t* mask = MASK ? b.allowed_mask + (size_t)row * (size_t)b.mask_ld : nullptr;
-  const float inv = inverse_temperature(b, row), c = inv * kLog2e;
+  const float inv = inverse_temperature(b, row), c = binary_scale(inv);
   const float cap = b.logit_softcap, inv_cap = CAP ? inverse_cap(cap) : 0.0f;
   const auto y_of = [&](float l) {
     if constexpr (CAP) return l == neg_inf() ? l : softcap_of(l, cap, inv_cap);
@@ -478,32 +479,23 @@ __global__ __launch_bounds__(kThreads, 4) void rows_kernel(Params p) {
       fetch(tile + 1u, next);
     }
     const Sums before_tile = sums;
-    float top = neg_inf();  // the thread's largest of the tile
-    bool odd = false;
 #pragma unroll
-    for (int e0 = 0; e0 < E; e0 += kStep) {
-#pragma unroll
-      for (int e = e0; e < e0 + kStep; ++e) {
-        if constexpr (DT == OXS_DTYPE_F32) v[e] = __uint_as_float(raw[e / G][e % G]);
-        else v[e] = __uint_as_float((e & 1) ? raw[e / G][(e % G) >> 1] & 0xffff0000u : raw[e / G][(e % G) >> 1] << 16);
-      }
-      float x;
+    for (int e = 0; e < E; ++e) {
+      if constexpr (DT == OXS_DTYPE_F32) v[e] = __uint_as_float(raw[e / G][e % G]);
+      else v[e] = __uint_as_float((e & 1) ? raw[e / G][(e % G) >> 1] & 0xffff0000u : raw[e / G][(e % G) >> 1] << 16);
       if constexpr (MASK) {
-#pragma unroll
-        for (int e = e0; e < e0 + kStep; ++e) {
-          const uint32_t in = (uint32_t)((int32_t)(keep << (31 - e)) >> 31);
-          v[e] = __uint_as_float((__float_as_uint(v[e]) & in) | (~in & 0xff800000u));
-        }
+        const uint32_t in = (uint32_t)((int32_t)(keep << (31 - e)) >> 31);
+        v[e] = __uint_as_float((__float_as_uint(v[e]) & in) | (~in & 0xff800000u));
       }
-      if constexpr (DT == OXS_DTYPE_BF16 && !MASK) x = largest_of_pairs(raw[e0 / G]);
-      else x = largest_of<kStep>(v + e0);
-      odd |= x != x;
-      top = fmaxf(top, x);
-      const float y = y_of(x);
-      if (__ballot(sums.behind(y, c))) sums.rebase(fmaxf(sums.ref, y), c);
-      sums.add<kStep>(v + e0, c, y_of);
-      __builtin_amdgcn_sched_barrier(0);  // nothing waits for the loads of later steps
     }
+    float top;  // the thread's largest of the tile
+    if constexpr (DT == OXS_DTYPE_BF16 && !MASK) top = largest_of_pairs<NG>(raw);
+    else top = largest_of<E>(v);
+    const bool odd = top != top;
+    // (Once per tile: once per eight logits of it took 116 us where this takes 106, 2048 rows of 128256 bf16 with 20
+    // alternatives.)
+    if (__ballot(sums.behind(y_of(top), c))) sums.rebase(fmaxf(sums.ref, y_of(top)), c);
+    sums.add<E>(v, c, y_of);
     const bool slow = __ballot(odd || sums.huge()) != 0;
     if (__builtin_expect(slow, 0)) {
       // NaNs among the logits may have hidden the largest, and a huge one (a mask of the type's lowest value, say)
@@ -749,7 +741,7 @@ __global__ __launch_bounds__(64) void merge_kernel(Params p) {
   for (uint32_t j = 0; j < kAhead; ++j) some[j] = count_of(j);
   const float want_l = __uint_as_float(counts[S * T + min(lane, max(T, 1u) - 1u)]);
   if (lane >= S) st = make_float4(neg_inf(), 0.0f, 0.0f, 0.0f);
-  const float inv = inverse_temperature(b, row), c = inv * kLog2e, cap = b.logit_softcap,
+  const float inv = inverse_temperature(b, row), c = binary_scale(inv), cap = b.logit_softcap,
               inv_cap = CAP ? inverse_cap(cap) : 0.0f;
   const auto y_of = [&](float l) {
     if constexpr (CAP) return l == neg_inf() ? l : softcap_of(l, cap, inv_cap);
