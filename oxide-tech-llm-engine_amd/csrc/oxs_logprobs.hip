@@ -16,13 +16,13 @@
 // threads with a logit above it hold candidates; ranks are counted tile by
 // tile against the given tokens' logits.
 //
-// What bounds it: long rows the read (512 rows of 262144 float32 86.6 us,
-// 6.2 TB/s, where a kernel that only reads takes 77), bf16 the vector unit
-// beside it (an exponential, four more operations and a comparison per logit,
-// twice the logits per byte: 2048 rows of 128256 101 us, 5.2 TB/s), decode
-// batches the start, the selection and the join (64 rows of 128256 float32, 20
-// alternatives: 20.0 us, of which the read alone takes 6.5 and the join 4),
-// one row two launches (32000 logits 9.6 us, 8.6 from a graph). A join in the
+// What bounds it: long rows the read (512 rows of 262144 float32 83 us,
+// 6.4 TB/s, where a kernel that only reads takes 77), bf16 the vector unit
+// beside it (an exponential and six more operations per logit, twice the
+// logits per byte: 2048 rows of 128256 93 us, 5.7 TB/s), decode batches the
+// start, the selection and the join (64 rows of 128256 float32, 20
+// alternatives: 18.8 us, of which the read alone takes 6.5 and the join 4),
+// one row two launches (32000 logits 9.1 us, 8.6 from a graph). A join in the
 // same launch, by the last workgroup of a row to finish, was no faster (16 rows
 // 10.6 us for 4.6 and 2.3; 64 rows equal).
 #include <hip/hip_runtime.h>

@@ -8,11 +8,11 @@
 //
 // What bounds it: large batches the read and write of y (1024 rows of 128256
 // float32 in 8 runs, rank 32: 236 us, 1.13 GB, 4.8 TB/s, a copy's rate; 64 rows,
-// 16 adapters of rank 16: 24.8 us, 4.7 TB/s). f16 weights their conversion and
+// 16 adapters of rank 16: 25 us, 4.6 TB/s). f16 weights their conversion and
 // the matrix instructions (256 rows of 151936, 4 adapters of rank 64, bf16 x and
 // y: 67 us for 210 MB; 48 at a copy's rate). Rows with an adapter each the chain
-// of loads (24 rows of 50257, float32 of rank 8: 17.7 us for 42 MB); one row the
-// two launches (32000 outputs, 4096 inputs: 8.9 us, 6.3 from a graph).
+// of loads (24 rows of 50257, float32 of rank 8: 17.5 us for 42 MB); one row the
+// two launches (32000 outputs, 4096 inputs: 9.0 us, 6.3 from a graph).
 //
 // Left out, measured: the first product on the matrix cores for rows that share
 // an adapter (1024 rows 48 to 90 us, 24 here) or four rows per wavefront (44);
