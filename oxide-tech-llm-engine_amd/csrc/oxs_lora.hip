@@ -4,7 +4,8 @@
 // shrink_kernel: v_b = s_a A_a x_b into the workspace, a wavefront per row and
 // one or four ranks. expand_kernel: y_b += B_a v_b on the matrix cores, 32
 // rows (few: 8) in order of adapter x 64 or 128 outputs per wavefront, for each
-// adapter among the rows in turn.
+// adapter among the rows in turn. single_kernel: both in one launch where there
+// is little to do, each workgroup with the whole of v for its outputs.
 //
 // What bounds it: large batches the read and write of y (1024 rows of 128256
 // float32 in 8 runs, rank 32: 236 us, 1.13 GB, 4.8 TB/s, a copy's rate; 64 rows,
@@ -206,11 +207,71 @@ __device__ __forceinline__ float wave_sum(float x) {
   return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), 63));
 }
 
-// One wavefront per (row, PER ranks): its lanes take eight values of x at a time. The loads of kAhead times 512 values
-// are on their way together, those of the first x before the row's adapter is known; lanes past the end load what
-// others do, for nothing: a load behind a branch would be waited for on its own (64 rows of 4096 values, 16 ranks: 6.8
-// us so, 4.7 here). The last workgroup of a row finds the row's place instead. Twice and four times kAhead: 7.7 and
-// 13.8 us for 7.3 (256 rows of 2048, f16 of rank 64), as fewer wavefronts fit.
+// The products of x with PER rows of A over one wavefront, whose lanes take eight values at a time. The loads of kAhead
+// times 512 values are on their way together; lanes past the end load what others do, for nothing: a load behind a
+// branch would be waited for on its own (64 rows of 4096 values, 16 ranks: 6.8 us so, 4.7 here). Twice and four times
+// kAhead: 7.7 and 13.8 us for 7.3 (256 rows of 2048, f16 of rank 64), as fewer wavefronts fit.
+template <int WT, int XT, int PER>
+struct Dots {
+  static constexpr uint32_t kAhead = PER == 1 ? 4 : WT == OXS_DTYPE_F32 ? 1 : 2, kStride = 512;
+  const Element<XT>* x;
+  uint32_t k, eights, lane;
+  Eight<XT> xv[kAhead];
+  float x_over;  // the values past the last eight, one in a lane
+  __device__ __forceinline__ uint32_t at(uint32_t i) const { return i < eights ? i : 0u; }
+  __device__ __forceinline__ void load_x(uint32_t i0) {
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; ++j) xv[j] = load_unaligned<XT>(x + at(i0 + lane * 8u + j * kStride));
+  }
+  // The first x, before the row's adapter is known.
+  __device__ __forceinline__ Dots(const Element<XT>* x_, uint32_t k_, uint32_t lane_)
+      : x(x_), k(k_), eights(k_ & ~7u), lane(lane_) {
+    if (eights) load_x(0);
+    const uint32_t over = eights + lane;
+    x_over = lane < 8u && over < k ? widen<XT>(x[over]) : 0.0f;
+  }
+  // Leaves x as it was found, for the next rows.
+  __device__ __forceinline__ float sum(const Element<WT>* w, bool again) {  // in lane p: row p's
+    const uint32_t kp = padded_k(k);
+    float s[PER];
+#pragma unroll
+    for (int p = 0; p < PER; ++p) s[p] = 0.0f;
+    for (uint32_t i0 = 0; i0 < eights;) {
+      Eight<WT> wv[kAhead][PER];
+#pragma unroll
+      for (uint32_t j = 0; j < kAhead; ++j)
+#pragma unroll
+        for (int p = 0; p < PER; ++p)
+          wv[j][p] = load_eight<WT>(w + (size_t)p * kp + at(i0 + lane * 8u + j * kStride));
+#pragma unroll
+      for (uint32_t j = 0; j < kAhead; ++j) {
+        const bool in = i0 + lane * 8u + j * kStride < eights;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = in ? xv[j][e] : 0.0f;
+#pragma unroll
+          for (int p = 0; p < PER; ++p) s[p] = __builtin_fmaf(wv[j][p][e], v, s[p]);
+        }
+      }
+      i0 += kAhead * kStride;
+      load_x(again && i0 >= eights ? 0u : i0);
+    }
+    if (eights < k && lane < 8u) {  // (the table's rows are padded to whole eights)
+#pragma unroll
+      for (int p = 0; p < PER; ++p)
+        s[p] = __builtin_fmaf(widen<WT>(w[(size_t)p * kp + eights + lane]), x_over, s[p]);
+    }
+    float v = 0.0f;
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const float all = wave_sum(s[p]);
+      if (lane == (uint32_t)p) v = all;
+    }
+    return v;
+  }
+};
+
+// One wavefront per (row, PER ranks). The last workgroup of a row finds the row's place instead.
 template <int WT, int XT, int PER>
 __global__ __launch_bounds__(kThreads) void shrink_kernel(oxs_lora_table t, oxs_lora_batch b, Place* places) {
   const uint32_t lane = threadIdx.x & 63u;
@@ -221,58 +282,13 @@ __global__ __launch_bounds__(kThreads) void shrink_kernel(oxs_lora_table t, oxs_
     place_row(b, row, a, rank_of(t, a), places);
     return;
   }
-  constexpr uint32_t kAhead = PER == 1 ? 4 : WT == OXS_DTYPE_F32 ? 1 : 2, kStride = 512;
-  const Element<XT>* x = (const Element<XT>*)b.x + (size_t)row * (size_t)b.x_ld;
-  const uint32_t eights = t.k & ~7u, from = lane * 8u;
-  const auto at = [&](uint32_t i) { return i < eights ? i : 0u; };
-  Eight<XT> xv[kAhead];
-  if (eights) {
-#pragma unroll
-    for (uint32_t j = 0; j < kAhead; ++j) xv[j] = load_unaligned<XT>(x + at(from + j * kStride));
-  }
-  // the values past the last eight, one in a lane
-  const uint32_t over = eights + lane;
-  const float x_over = lane < 8u && over < t.k ? widen<XT>(x[over]) : 0.0f;
+  Dots<WT, XT, PER> dots((const Element<XT>*)b.x + (size_t)row * (size_t)b.x_ld, t.k, lane);
   const uint32_t rank = rank_of(t, a), all_blocks = rank_blocks(t.max_rank);
   // With a rank per wavefront the weights are not waited for until the adapter's rank is known: a slot has room for
   // max_rank whatever it holds.
   if (PER == 1 ? a >= t.max_adapters : r0 >= rank_blocks(rank) * kBlock) return;
   const float scale = t.scales[a];
-  const uint32_t kp = padded_k(t.k);
-  const Element<WT>* w = (const Element<WT>*)t.a + (size_t)a * a_elements(t) + (size_t)r0 * kp;
-  float s[PER];
-#pragma unroll
-  for (int p = 0; p < PER; ++p) s[p] = 0.0f;
-  for (uint32_t i0 = 0; i0 < eights;) {
-    Eight<WT> wv[kAhead][PER];
-#pragma unroll
-    for (uint32_t j = 0; j < kAhead; ++j)
-#pragma unroll
-      for (int p = 0; p < PER; ++p) wv[j][p] = load_eight<WT>(w + (size_t)p * kp + at(i0 + from + j * kStride));
-#pragma unroll
-    for (uint32_t j = 0; j < kAhead; ++j) {
-      const bool in = i0 + from + j * kStride < eights;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = in ? xv[j][e] : 0.0f;
-#pragma unroll
-        for (int p = 0; p < PER; ++p) s[p] = __builtin_fmaf(wv[j][p][e], v, s[p]);
-      }
-    }
-    i0 += kAhead * kStride;
-#pragma unroll
-    for (uint32_t j = 0; j < kAhead; ++j) xv[j] = load_unaligned<XT>(x + at(i0 + from + j * kStride));
-  }
-  if (eights < t.k && lane < 8u) {  // (the table's rows are padded to whole eights)
-#pragma unroll
-    for (int p = 0; p < PER; ++p) s[p] = __builtin_fmaf(widen<WT>(w[(size_t)p * kp + over]), x_over, s[p]);
-  }
-  float v = 0.0f;  // lane p: rank r0 + p's
-#pragma unroll
-  for (int p = 0; p < PER; ++p) {
-    const float sum = wave_sum(s[p]);
-    if (lane == (uint32_t)p) v = sum;
-  }
+  const float v = dots.sum((const Element<WT>*)t.a + (size_t)a * a_elements(t) + (size_t)r0 * padded_k(t.k), false);
   // ranks past the adapter's, up to the block's end, are zero
   if (lane < PER && r0 + lane < rank_blocks(rank) * kBlock)
     store_value(b.workspace, row, all_blocks, r0 + lane, r0 + lane < rank ? v * scale : 0.0f);
@@ -538,6 +554,83 @@ __global__ __launch_bounds__(kThreads, RR == 4 || (PF == 1 && WT != OXS_DTYPE_F3
   }
 }
 
+// ---------------------------------------------------------------- few rows: both products in one launch
+
+// One workgroup: a row and kWaves * 128 outputs. It computes all of the row's v for itself, with B's first weights and
+// y on their way meanwhile; lane (n, g) of a wavefront then has half g of the ranks of a block for outputs 4 n to
+// 4 n + 3.
+template <int WT, int XT, int YT>
+__global__ __launch_bounds__(kThreads) void single_kernel(oxs_lora_table t, oxs_lora_batch b) {
+  const uint32_t lane = threadIdx.x & 63u, n = lane & 31u, g = lane >> 5;
+  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t row = blockIdx.y, col = blockIdx.x * kWaves + wave;
+  __shared__ float s_v[OXS_LORA_MAX_RANK];
+  const uint32_t a = b.adapters[row];
+  Dots<WT, XT, 4> dots((const Element<XT>*)b.x + (size_t)row * (size_t)b.x_ld, t.k, lane);
+  const uint32_t rank = rank_of(t, a), blocks = rank_blocks(rank);
+  if (rank == 0u) return;
+  const float scale = t.scales[a];
+  const bool mine = (uint64_t)col * kGroup < t.m;  // this wavefront has outputs
+  const Element<WT>* w = (const Element<WT>*)t.b + (size_t)a * b_elements(t) +
+                         (size_t)(mine ? col : 0u) * rank_blocks(t.max_rank) * (kBlock * kGroup) + n * 8u;
+  Eight<WT> wv[4];
+  // A half that holds no rank takes the other's weights, to be multiplied by values of 0.
+  const auto fetch = [&](uint32_t block) {
+    const Element<WT>* p = w + (size_t)block * (kBlock * kGroup) + (block * kBlock + 8u * g < rank ? g * 1024u : 0u);
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) wv[tt] = load_eight<WT>(p + tt * 256u);
+  };
+  fetch(0);
+  using YE = Element<YT>;
+  const uint32_t out = col * kGroup + 4u * n;
+  YE* y = (YE*)b.y + (size_t)row * (size_t)b.y_ld;
+  struct Vec {
+    YE e[4];
+  } old;
+  const bool inside = (uint64_t)(col + 1u) * kGroup <= t.m;
+  if (inside) {
+    __builtin_memcpy(&old, y + out, sizeof(Vec));
+  } else {
+#pragma unroll
+    for (uint32_t tt = 0; tt < 4; ++tt) old.e[tt] = y[min((uint64_t)out + tt, (uint64_t)t.m - 1u)];
+  }
+  const Element<WT>* wa = (const Element<WT>*)t.a + (size_t)a * a_elements(t) + (size_t)(wave * 4u) * padded_k(t.k);
+  for (uint32_t block = 0; block < blocks; ++block) {
+    const float v = dots.sum(wa + (size_t)block * kBlock * padded_k(t.k), block + 1u < blocks);
+    const uint32_t r = block * kBlock + wave * 4u + lane;
+    if (lane < 4u) s_v[r] = r < rank ? v * scale : 0.0f;
+  }
+  __syncthreads();
+  if (!mine) return;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t block = 0; block < blocks; ++block) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = s_v[block * kBlock + g * 8u + j];
+    const Eight<WT> now[4] = {wv[0], wv[1], wv[2], wv[3]};
+    fetch(min(block + 1u, blocks - 1u));
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[tt] = __builtin_fmaf(now[tt][j], v[j], acc[tt]);
+  }
+  Vec z;
+#pragma unroll
+  for (int tt = 0; tt < 4; ++tt) {
+    const float sum = widen<YT>(old.e[tt]) + (acc[tt] + __shfl_xor(acc[tt], 32));
+    if constexpr (YT == OXS_DTYPE_BF16) z.e[tt] = (YE)narrow2(sum, 0.0f);
+    else z.e[tt] = __float_as_uint(sum);
+  }
+  if (g) return;
+  if (inside) {
+    __builtin_memcpy(y + out, &z, sizeof(Vec));
+  } else {
+#pragma unroll
+    for (uint32_t tt = 0; tt < 4; ++tt)
+      if ((uint64_t)out + tt < t.m) y[out + tt] = z.e[tt];
+  }
+}
+
 static bool known(int32_t dt, bool half) {
   return dt == OXS_DTYPE_F32 || dt == OXS_DTYPE_BF16 || (half && dt == OXS_DTYPE_F16);
 }
@@ -622,6 +715,24 @@ extern "C" int oxs_lora_add(const oxs_lora_table* table, const oxs_lora_batch* b
   const auto even = [&](const void* p, int64_t ld, uint32_t es, uint32_t to) {
     return aligned(p, to) && (b.batch == 1 || ((uint64_t)ld * es) % to == 0);
   };
+  // Both products in one launch while no workgroup has much of A to read, all together have not, and they are few. One
+  // launch and two, us, replayed from a graph, rank 16 in bf16: one row of 32000 outputs, 896 inputs 3.3 and 5.9, 4096
+  // 4.5 and 6.2, 8192 6.0 and 7.0, 4096 of rank 64 10.6 and 7.5; 128256 outputs, 4096 inputs, 1 row 4.8 and 7.0, 2 rows
+  // 6.8 and 7.7, 4 rows 10.7 and 8.8; 512 inputs, 64 rows of 8000 6.0 and 6.8, 200 rows 14.7 and 8.8.
+  const uint32_t singles = (t.m + kWaves * kGroup - 1u) / (kWaves * kGroup);
+  const uint64_t a_bytes = (uint64_t)blocks * kBlock * padded_k(t.k) * size_of(t.dtype);
+  const uint64_t groups = (uint64_t)b.batch * singles;
+  if (groups <= 1024u && a_bytes <= (256u << 10) && groups * a_bytes <= (80u << 20)) {
+    by_weights(t.dtype, [&](auto wt) {
+      by_values(b.x_dtype, [&](auto xt) {
+        by_values(b.y_dtype, [&](auto yt) {
+          hipLaunchKernelGGL((single_kernel<decltype(wt)::value, decltype(xt)::value, decltype(yt)::value>),
+                             dim3(singles, b.batch), dim3(kThreads), 0, st, t, b);
+        });
+      });
+    });
+    return launched();
+  }
   by_weights(t.dtype, [&](auto wt) {
     constexpr int WT = decltype(wt)::value;
     by_values(b.x_dtype, [&](auto xt) {

@@ -218,6 +218,54 @@ def test_batches_around_the_kernels_own_sizes(torch_gpu, batch, ranks, w, order)
     check(y, want, bound, f"{batch} {order}")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["mixed", "packed"])
+@pytest.mark.parametrize("batch,m,k,ranks,w,xd,yd", CASES)
+def test_small_tables_slots_for_large_ranks(torch_gpu, batch, m, k, ranks, w, xd, yd, order):
+    # with room for rank 256 and more inputs the same calls take two launches and tiles of 8 rows
+    t = torch_gpu
+    k += 640
+    x, y, ad, dt, g = make(t, batch * 17 + m, batch, m, k, ranks, w)
+    kinds = {"f32": t.float32, "bf16": t.bfloat16}
+    x = x.to(kinds[xd])
+    flat = t.full((batch, m + batch % 5), 7.0, dtype=kinds[yd], device="cuda")  # y of many alignments
+    yv = flat[:, :m]
+    yv.copy_(y)
+    ids = t.randint(-1, len(ranks) + 1, (batch,), generator=g, device="cuda", dtype=t.int32)
+    if batch == 1:
+        ids[:] = 0
+    if order == "packed":
+        ids = ids.sort().values
+    want, bound = reference(yv, x, ids, ad, yd == "bf16")
+    before = flat.clone()
+    lora = table(t, m, k, ranks, ad, dt, batch, max_rank=256)
+    lora.add(yv, x, ids)
+    check(yv, want, bound, f"{batch} x {m}")
+    idle = t.tensor([int(i) not in ad for i in ids.tolist()], device="cuda")
+    assert t.equal(flat[idle], before[idle]) and t.equal(flat[:, m:], before[:, m:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [3, 40])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_infinities_stay_with_their_rows_in_small_tiles(torch_gpu, batch, dtype):
+    t = torch_gpu
+    m, k, ranks = 700, 1000, [16, 16, 3]
+    x, y, ad, dt, g = make(t, 78, batch, m, k, ranks, dtype)
+    ids = t.randint(0, 3, (batch,), generator=g, device="cuda", dtype=t.int32)
+    ids[:3] = t.tensor([0, 1, 2])
+    want, bound = reference(y, x, ids, ad)
+    bad = ad | {1: (ad[1][0].clone(), ad[1][1].clone(), ad[1][2])}
+    bad[1][0][3, 5] = float("inf")
+    bad[1][1][2, 4] = float("nan")
+    x[0, 999] = float("nan")  # the last value of an odd eight
+    table(t, m, k, ranks, bad, dt, batch, max_rank=256).add(y, x, ids)
+    fine = ids != 1
+    fine[0] = False
+    check(y[fine], want[fine], bound[fine])
+    assert bool(y[0].isnan().all()) and not bool(y[ids == 1].isfinite().any())
+
+
 LARGE = [
     # tiles of 32 rows: batch, m, k, ranks of the slots, weights, x, y, extra elements between y's rows
     (33, 70001, 24, [16, 3], "f32", "f32", "f32", 0),
