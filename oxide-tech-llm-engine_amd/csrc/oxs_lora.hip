@@ -12,15 +12,18 @@
 // 16 adapters of rank 16: 25 us, 4.6 TB/s). f16 weights their conversion and
 // the matrix instructions (256 rows of 151936, 4 adapters of rank 64, bf16 x and
 // y: 67 us for 210 MB; 48 at a copy's rate). Rows with an adapter each the chain
-// of loads (24 rows of 50257, float32 of rank 8: 17.5 us for 42 MB); one row the
-// two launches (32000 outputs, 4096 inputs: 9.0 us, 6.3 from a graph).
+// of loads (24 rows of 50257, float32 of rank 8: 17.3 us for 42 MB); one row the
+// launch (32000 outputs, 4096 inputs: 5.5 us, 4.5 from a graph).
 //
 // Left out, measured: the first product on the matrix cores for rows that share
 // an adapter (1024 rows 48 to 90 us, 24 here) or four rows per wavefront (44);
 // row tiles of 64 (prompts 276 us for 230, f16 98 for 76); v through LDS (one row
 // 7.0 us for 5.3); three or four pairs of operands on their way (registers
 // spill: prompts 375 us for 232); row tiles side by side (prompts 259 us for 231)
-// or in chunks of 32 to 256 ranges of outputs (within 5% either way).
+// or in chunks of 32 to 256 ranges of outputs (within 5% either way); tiles of 2
+// to 4 rows, or the second product row by row on the vector unit, where every
+// row has an adapter of its own (14 us for 19 in the case above, but 42 for 13
+// where 32 rows share one, which the host cannot tell).
 //
 // The matrix cores take bf16. A float is the sum of three bf16 (each the
 // nearest to what is left of it: 2^-9 of it remains after one, 2^-18 after
