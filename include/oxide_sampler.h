@@ -632,7 +632,7 @@ size_t oxs_lora_workspace_bytes(const oxs_lora_table* table, uint32_t batch);
  * adapters[b]; y of a row whose slot is empty or >= max_adapters is neither
  * read nor written. Weights, x and A x enter their products with all of their
  * bits (a weight of B or a value of A x beyond the largest bfloat16, 3.39e38,
- * counts as infinite) and sums are in 32 bits; the result is added to y in 32
+ * may count as infinite) and sums are in 32 bits; the result is added to y in 32
  * bits and rounded to y_dtype once. Rows may have any adapters in any order;
  * the rows of an adapter share its reads. Repeated calls give equal bits. y
  * must not overlap the other arrays.

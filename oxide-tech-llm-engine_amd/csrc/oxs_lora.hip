@@ -11,7 +11,7 @@
 // float32 in 8 runs, rank 32: 236 us, 1.13 GB, 4.8 TB/s, a copy's rate; 64 rows,
 // 16 adapters of rank 16: 25 us, 4.6 TB/s). f16 weights their conversion and
 // the matrix instructions (256 rows of 151936, 4 adapters of rank 64, bf16 x and
-// y: 67 us for 210 MB; 48 at a copy's rate). Rows with an adapter each the chain
+// y: 67 us for 210 MB; 43 at a copy's rate). Rows with an adapter each the chain
 // of loads (24 rows of 50257, float32 of rank 8: 17.3 us for 42 MB); one row the
 // launch (32000 outputs, 4096 inputs: 5.5 us, 4.5 from a graph).
 //
